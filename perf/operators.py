@@ -21,29 +21,29 @@ TYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.
 def listed():
     return [
         # the mapping network's own norm at the batch of one interactive request (z_dim 512): a call's latency
-        {"name": "norm z, 4 rows", "op": "norm", "rows": 4, "cols": 512, "dtype": "float32", "residual": False, "weight": False},
+        {"name": "norm z 4 rows", "op": "norm", "rows": 4, "cols": 512, "dtype": "float32", "residual": False, "weight": False},
         # many narrow rows of a width that no vector load divides: ragged features
-        {"name": "norm odd, 10001 x 1031", "op": "norm", "rows": 10001, "cols": 1031, "dtype": "float16", "residual": False, "weight": True},
+        {"name": "norm odd 10001x1031", "op": "norm", "rows": 10001, "cols": 1031, "dtype": "float16", "residual": False, "weight": True},
         # a wide layer's residual stream, all of a large batch: bandwidth
-        {"name": "norm wide, 16384 x 4096", "op": "norm", "rows": 16384, "cols": 4096, "dtype": "bfloat16", "residual": True, "weight": True},
+        {"name": "norm wide 16384x4096", "op": "norm", "rows": 16384, "cols": 4096, "dtype": "bfloat16", "residual": True, "weight": True},
         # first layer of the mapping network for one latent (z 512 + embedded camera 512 -> 512): latency
-        {"name": "mm mapping, 1 row", "op": "mm", "rows": 1, "out": 512, "cols": 1024, "dtype": "float32", "lrelu": True, "bias": True},
+        {"name": "mm mapping 1 row", "op": "mm", "rows": 1, "out": 512, "cols": 1024, "dtype": "float32", "lrelu": True, "bias": True},
         # the same layer over the latents that estimate the mean w
-        {"name": "mm mapping, 10000 rows", "op": "mm", "rows": 10000, "out": 512, "cols": 1024, "dtype": "float32", "lrelu": True, "bias": True},
+        {"name": "mm mapping 10000 rows", "op": "mm", "rows": 10000, "out": 512, "cols": 1024, "dtype": "float32", "lrelu": True, "bias": True},
         # few rows against large weights: reading the weights once is all there is
-        {"name": "mm stream, 16 x 8192 x 8192", "op": "mm", "rows": 16, "out": 8192, "cols": 8192, "dtype": "bfloat16", "lrelu": False, "bias": False},
+        {"name": "mm stream 16x8192x8192", "op": "mm", "rows": 16, "out": 8192, "cols": 8192, "dtype": "bfloat16", "lrelu": False, "bias": False},
         # a square product that fills the card
-        {"name": "mm square, 4096", "op": "mm", "rows": 4096, "out": 4096, "cols": 4096, "dtype": "bfloat16", "lrelu": False, "bias": True},
+        {"name": "mm square 4096", "op": "mm", "rows": 4096, "out": 4096, "cols": 4096, "dtype": "bfloat16", "lrelu": False, "bias": True},
         # the largest, with edges that end inside a tile on both sides
-        {"name": "mm large, 8191 x 8190 x 8192", "op": "mm", "rows": 8191, "out": 8190, "cols": 8192, "dtype": "float16", "lrelu": False, "bias": False},
+        {"name": "mm large 8191x8190x8192", "op": "mm", "rows": 8191, "out": 8190, "cols": 8192, "dtype": "float16", "lrelu": False, "bias": False},
         # appearance editing: mean and deviation of one plane set are the leaves
-        {"name": "clip statistics, 2 x 96", "op": "clip", "count": 2, "total": 192, "dtype": "float32", "clipped": True},
+        {"name": "clip statistics 2x96", "op": "clip", "count": 2, "total": 192, "dtype": "float32", "clipped": True},
         # geometry editing: the planes of four views (4 x 96 x 256 x 256) twice
-        {"name": "clip planes, 50.3M", "op": "clip", "count": 2, "total": 50331648, "dtype": "float32", "clipped": True},
+        {"name": "clip planes 50.3M", "op": "clip", "count": 2, "total": 50331648, "dtype": "float32", "clipped": True},
         # the same size of one view, inside the limit: nothing is to be written
-        {"name": "clip idle, 6.3M", "op": "clip", "count": 1, "total": 6291456, "dtype": "float32", "clipped": False},
+        {"name": "clip idle 6.3M", "op": "clip", "count": 1, "total": 6291456, "dtype": "float32", "clipped": False},
         # all parameters of a generator (180 tensors, 30 M values), half of them held in bfloat16
-        {"name": "clip model, 180 tensors", "op": "clip", "count": 180, "total": 30000000, "dtype": "mixed", "clipped": True},
+        {"name": "clip model 180 tensors", "op": "clip", "count": 180, "total": 30000000, "dtype": "mixed", "clipped": True},
     ]
 
 
