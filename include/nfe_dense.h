@@ -198,6 +198,27 @@ int nfe_resize_bilinear_backward(const float* grad_out, int n, int h, int w, int
 int nfe_bias_act_backward(const float* out, const float* grad, const float* grad_rgb, const float* rgb_w, const float* rgb_s, int rgb_k,
                           const float* scale, float gain, float clamp, int n, long long pixels, int c, float* dst, nfe_stream_t stream);
 
+/* ---- element types of the entry points below (ABI v16) */
+#define NFE_F32 0
+#define NFE_BF16 1
+#define NFE_F16 2
+
+/* ---- global gradient norm over a list of tensors, and clipping in place (ABI v16; editing.optimize_planes' max_grad_norm) ----
+ *   norm = sqrt(sum over all tensors of g^2)  (NFE_NORM_2; fp64 sums)   or   max |g|  (NFE_NORM_MAX; a NaN anywhere gives NaN)
+ *   nfe_grad_clip: g <- g * min(1, max_norm / (norm + 1e-6)), rounded once to g's type; nothing is written where the factor is 1, and
+ *   a NaN norm makes every gradient NaN (torch.nn.utils.clip_grad_norm_'s behaviour).
+ * data / n / dtype are HOST arrays of `count` entries: device pointer (aligned to its element), number of contiguous elements (0 is
+ * allowed, at most 2^37), NFE_F32 / NFE_BF16 / NFE_F16.  Entries of one nfe_grad_clip list must not share memory (NFE_EINVAL).
+ * norm: one device float.  workspace: nfe_grad_workspace_bytes(count) device bytes, 8-byte aligned, no initial contents needed.
+ * Same list, same bits: partial sums are joined in a fixed order.  May be captured into a graph (the list is baked in). */
+#define NFE_NORM_2 0
+#define NFE_NORM_MAX 1
+uint64_t nfe_grad_workspace_bytes(int count);
+int nfe_grad_norm(const uint64_t* data, const int64_t* n, const int32_t* dtype, int count, int norm_type, float* norm, void* workspace,
+                  uint64_t workspace_bytes, nfe_stream_t stream);
+int nfe_grad_clip(const uint64_t* data, const int64_t* n, const int32_t* dtype, int count, int norm_type, float max_norm, float* norm,
+                  void* workspace, uint64_t workspace_bytes, nfe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,7 +7,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # NFE_RENDER_LIB lets tools/ load an experimental build of the same ABI (kernel ablations)
 LIB_PATH = os.environ.get("NFE_RENDER_LIB") or os.path.join(_HERE, "libnfe_render.so")
 
-NFE_ABI_VERSION = 15
+NFE_ABI_VERSION = 16
 NFE_MAX_SAMPLES = 256
 NFE_DECODER_PACKED_FLOATS = 4 * 2048 + 64 + 64 + 32 + 32 + 8192
 NFE_DECODER_CROSS_FLOATS = 2048
@@ -91,6 +91,8 @@ class DemodGroup(ctypes.Structure):
     _fields_ = [("styles", FP), ("wsq", FP), ("dcoef", FP), ("cin", c_int32), ("cout", c_int32), ("styles_norm", FP)]
 
 
+NFE_F32, NFE_BF16, NFE_F16 = 0, 1, 2
+NFE_NORM_2, NFE_NORM_MAX = 0, 1
 NFE_MAX_GROUPS = 32
 NFE_CONV_BF16X3, NFE_CONV_BF16, NFE_CONV_F16 = 0, 1, 2
 NFE_CONV_3X3, NFE_CONV_3X3_UP2, NFE_CONV_1X1 = 0, 1, 2
@@ -142,6 +144,9 @@ _SIGNATURES = {
     "nfe_resize_bilinear_backward": (c_int, [FP, c_int, c_int, c_int, c_int, c_int, c_int, c_int, FP, c_void_p]),
     "nfe_upfirdn2d_polyphase": (c_int, [FP, c_int, c_int, c_int, c_int, c_int, c_int, c_float, FP, c_void_p]),
     "nfe_bias_act_backward": (c_int, [FP, FP, FP, FP, FP, c_int, FP, c_float, c_float, c_int, c_int64, c_int, FP, c_void_p]),
+    "nfe_grad_workspace_bytes": (c_uint64, [c_int]),
+    "nfe_grad_norm": (c_int, [POINTER(c_uint64), POINTER(c_int64), POINTER(c_int32), c_int, c_int, FP, FP, c_uint64, c_void_p]),
+    "nfe_grad_clip": (c_int, [POINTER(c_uint64), POINTER(c_int64), POINTER(c_int32), c_int, c_int, c_float, FP, FP, c_uint64, c_void_p]),
     "nfe_point_query": (c_int, [FP, FP, c_int, c_int, c_int64, FP, FP, FP, FP, FP, c_int, FP, c_int, c_int, c_float,
                                 FP, FP, FP, c_float, c_uint64, FP, c_void_p]),
 }

@@ -1,6 +1,7 @@
 // Memory-bound helper kernels around the render core (gfx950): ray sampler, plane statistics,
-// per-channel affine, NCHW -> gather-layout pack, decoder weight packing.
+// per-channel affine, NCHW -> gather-layout pack, decoder weight packing, gradient norm and clipping (nfe_grad.h).
 #include "nfe_common.h"
+#include "nfe_grad.h"
 
 namespace nfe {
 

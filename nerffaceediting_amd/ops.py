@@ -492,3 +492,74 @@ def point_query(planes_geo, planes_app, decoder_packed, coords, box_warp, affine
                                        _ptr(_dev(decoder_cross, "decoder_cross", (_lib.NFE_DECODER_CROSS_FLOATS,)) if decoder_cross is not None else None), _stream()),
                    "nfe_point_query")
     return {"rgb": rgb, "sigma": sigma, "seg": seg}
+
+
+_GRAD_TYPES = {torch.float32: _lib.NFE_F32, torch.bfloat16: _lib.NFE_BF16, torch.float16: _lib.NFE_F16}
+_NORM_TYPES = {2: _lib.NFE_NORM_2, float("inf"): _lib.NFE_NORM_MAX}
+
+
+def _is_dense(t):
+    """Whether the elements of t fill one stretch of memory, in whatever order of the axes."""
+    expected = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _grad_list(what, tensors, writes):
+    ts = [tensors] if isinstance(tensors, torch.Tensor) else [t for t in tensors if t is not None]
+    if not ts:
+        raise ValueError(f"{what}: no tensors")
+    for i, t in enumerate(ts):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: expected torch.Tensors, got {type(t)}")
+        if not t.is_cuda:
+            raise RuntimeError(f"{what}: tensor {i} is on {t.device}; this path runs only on the GPU (no CPU fallback)")
+        if t.dtype not in _GRAD_TYPES:
+            raise RuntimeError(f"{what}: tensor {i} is {t.dtype}; expected float32, bfloat16 or float16")
+        if t.requires_grad and writes and torch.is_grad_enabled():
+            raise RuntimeError(f"{what}: tensor {i} is part of an autograd graph; it is written in place (detach it, or use torch.no_grad())")
+        if not t.is_contiguous() and t.numel() and not _is_dense(t):
+            if writes:
+                raise RuntimeError(f"{what}: tensor {i} (shape {list(t.shape)}, strides {list(t.stride())}) does not fill one stretch of memory")
+            ts[i] = t.detach().contiguous()
+    dev = ts[0].device
+    if any(t.device != dev for t in ts):
+        raise RuntimeError(f"{what}: the tensors are on several devices")
+    return ts, dev
+
+
+def _grad_call(what, tensors, norm_type, max_norm=None):
+    lib = _lib.load()
+    if norm_type not in _NORM_TYPES:
+        raise ValueError(f"{what}: norm_type must be 2 or inf, got {norm_type!r}")
+    ts, dev = _grad_list(what, tensors, max_norm is not None)
+    n = len(ts)
+    data = (ctypes.c_uint64 * n)(*[t.data_ptr() for t in ts])
+    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in ts])
+    types = (ctypes.c_int32 * n)(*[_GRAD_TYPES[t.dtype] for t in ts])
+    norm = torch.empty((), device=dev)
+    with torch.cuda.device(dev):
+        ws = _workspace(dev, lib.nfe_grad_workspace_bytes(n))
+        tail = (_ptr(norm), _ptr(ws), ws.numel(), _stream())
+        if max_norm is None:
+            _lib.check(lib.nfe_grad_norm(data, sizes, types, n, _NORM_TYPES[norm_type], *tail), "nfe_grad_norm")
+        else:
+            _lib.check(lib.nfe_grad_clip(data, sizes, types, n, _NORM_TYPES[norm_type], float(max_norm), *tail), "nfe_grad_clip")
+            torch.autograd.graph.increment_version(ts)
+    return norm
+
+
+def grad_norm(tensors, norm_type=2):
+    """nfe_grad_norm: the norm of all gradients in `tensors` (fp32 / bf16 / fp16 GPU tensors of one device, any mix, any strides; None
+    entries are skipped) as one vector -> fp32 scalar tensor on their device.  norm_type 2 (sums in fp64) or inf."""
+    return _grad_call("grad_norm", tensors, norm_type)
+
+
+def clip_grad_norm(tensors, max_norm, norm_type=2):
+    """nfe_grad_clip: scale the gradients in `tensors` in place by min(1, max_norm / (norm + 1e-6)) and return the norm before that
+    (fp32 scalar tensor; no synchronisation) - torch.nn.utils.clip_grad_norm_ on gradient tensors.  A norm that is NaN makes every
+    gradient NaN.  The tensors must not share memory and each must fill one stretch of memory (a transposed tensor does)."""
+    return _grad_call("clip_grad_norm", tensors, norm_type, max_norm)

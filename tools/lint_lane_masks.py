@@ -40,7 +40,7 @@ BLOCK_END = re.compile(r"^\s*(s_cbranch|s_branch|s_endpgm|s_setpc|s_swappc)|^[.\
 
 def assemble(src, outdir, extra=()):
     out = os.path.join(outdir, os.path.basename(src) + ".s")
-    deps = [src, os.path.join(CSRC, "nfe_common.h")]
+    deps = [src] + [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".h")]
     if os.path.exists(out) and not extra and all(os.path.getmtime(out) >= os.path.getmtime(d) for d in deps):
         return out
     cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-fno-gpu-rdc", "-I" + os.path.join(ROOT, "include"),
