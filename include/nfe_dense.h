@@ -219,6 +219,48 @@ int nfe_grad_norm(const uint64_t* data, const int64_t* n, const int32_t* dtype, 
 int nfe_grad_clip(const uint64_t* data, const int64_t* n, const int32_t* dtype, int count, int norm_type, float max_norm, float* norm,
                   void* workspace, uint64_t workspace_bytes, nfe_stream_t stream);
 
+/* ---- 8-bit rows: e4m3 values (OCP, largest 448) with one fp32 scale for every 128 columns (ABI v16) ----------------------------
+ *   h = x + residual                      (residual NULL: h = x)
+ *   y = h * rsqrt(mean(h^2) + eps) * weight   (nfe_rms_norm_fp8; weight NULL: ones; networks_stylegan2.py:24-26 with weight NULL, eps 1e-8)
+ *   y = x                                 (nfe_quantize_fp8)
+ *   per 128 columns: a = max(max |y|, 1e-30), scale = a / 448, q = e4m3(y / scale), round to nearest even
+ * x, residual, h: [rows, cols] of `dtype`, contiguous; h (required with residual, and only then) gets x + residual rounded to `dtype` - the
+ * norm uses the sum before that rounding.  weight: [cols] fp32.  q: [rows][q_stride] bytes, q_stride >= cols rounded up to 128 and a multiple
+ * of 8; columns from `cols` up to that width are written as zeros.  scale of row r, block b: scale[r * scale_row_stride + b *
+ * scale_block_stride] (block-major, scale_row_stride = 1, is what nfe_fp8_matmul reads fastest).  A NaN or an infinity makes every value
+ * of its block read as NaN.  Sums and products are fp32. */
+int nfe_rms_norm_fp8(const void* x, const void* residual, const float* weight, int dtype, int64_t rows, int cols, float eps, void* h, void* q,
+                     int64_t q_stride, float* scale, int64_t scale_row_stride, int64_t scale_block_stride, nfe_stream_t stream);
+int nfe_quantize_fp8(const void* x, int dtype, int64_t rows, int cols, void* q, int64_t q_stride, float* scale, int64_t scale_row_stride,
+                     int64_t scale_block_stride, nfe_stream_t stream);
+
+/* ---- 8-bit weights: e4m3 with one fp32 scale for every 128 x 128 block of [n, k] (ABI v16) ------------------------------------
+ * packed: nfe_fp8_weight_bytes(n, k) bytes, 16-byte aligned, the matrix instruction's operand order (opaque).  scale [ceil(n/128)][ceil(k/128)].
+ * nfe_fp8_weight_quantize rounds w [n, k] (`dtype`) and multiplies the scales by gain (FullyConnectedLayer's weight_gain);
+ * nfe_fp8_weight_pack lays out values that are e4m3 already (q [n, k] bytes; their scales stay the caller's). */
+uint64_t nfe_fp8_weight_bytes(int n, int k);
+int nfe_fp8_weight_quantize(const void* w, int dtype, int n, int k, float gain, void* packed, float* scale, nfe_stream_t stream);
+int nfe_fp8_weight_pack(const void* q, int n, int k, void* packed, nfe_stream_t stream);
+
+/* ---- FullyConnectedLayer.forward on 8-bit rows and weights (ABI v16; networks_stylegan2.py:114-127) ---------------------------
+ * out[i, o] = act( sum_b scale[i, b] w_scale[o / 128, b] sum_{c in block b} q[i, c] w[o, c]  +  bias[o] * bias_gain ),
+ * act = linear or lrelu(0.2) * sqrt(2); block sums are scaled and added in fp32 and rounded once to out_dtype.  A block's sum over its 128
+ * columns is fp32-grade for NFE_F32 outputs (e4m3 widened to bf16 operands, exact products); for NFE_BF16 / NFE_F16 outputs it is the
+ * 8-bit matrix instruction's, off by less than 7 2^-13 sum|products| (1.5e-5 of the result for normally distributed operands).
+ * q: [m][q_stride] bytes, 16-byte aligned rows, ceil(k/128)*128 columns (those from k on must be zero or meet zero weights: any finite
+ * value).  out: [m, n] contiguous. */
+typedef struct nfe_fp8_matmul_args {
+    uint32_t struct_size;
+    int32_t m, n, k;
+    const void* q; int64_t q_stride;
+    const float* scale; int64_t scale_row_stride, scale_block_stride;
+    const void* packed; const float* w_scale;
+    const float* bias; float bias_gain;           /* bias: [n] or NULL */
+    int32_t lrelu, out_dtype;
+    void* out;
+} nfe_fp8_matmul_args;
+int nfe_fp8_matmul(const nfe_fp8_matmul_args* args, nfe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -91,6 +91,15 @@ class DemodGroup(ctypes.Structure):
     _fields_ = [("styles", FP), ("wsq", FP), ("dcoef", FP), ("cin", c_int32), ("cout", c_int32), ("styles_norm", FP)]
 
 
+class Fp8MatmulArgs(ctypes.Structure):
+    """Mirror of ``nfe_fp8_matmul_args``."""
+    _fields_ = [
+        ("struct_size", c_uint32), ("m", c_int32), ("n", c_int32), ("k", c_int32),
+        ("q", FP), ("q_stride", c_int64), ("scale", FP), ("scale_row_stride", c_int64), ("scale_block_stride", c_int64),
+        ("packed", FP), ("w_scale", FP), ("bias", FP), ("bias_gain", c_float), ("lrelu", c_int32), ("out_dtype", c_int32), ("out", FP),
+    ]
+
+
 NFE_F32, NFE_BF16, NFE_F16 = 0, 1, 2
 NFE_NORM_2, NFE_NORM_MAX = 0, 1
 NFE_MAX_GROUPS = 32
@@ -147,6 +156,12 @@ _SIGNATURES = {
     "nfe_grad_workspace_bytes": (c_uint64, [c_int]),
     "nfe_grad_norm": (c_int, [POINTER(c_uint64), POINTER(c_int64), POINTER(c_int32), c_int, c_int, FP, FP, c_uint64, c_void_p]),
     "nfe_grad_clip": (c_int, [POINTER(c_uint64), POINTER(c_int64), POINTER(c_int32), c_int, c_int, c_float, FP, FP, c_uint64, c_void_p]),
+    "nfe_rms_norm_fp8": (c_int, [FP, FP, FP, c_int, c_int64, c_int, c_float, FP, FP, c_int64, FP, c_int64, c_int64, c_void_p]),
+    "nfe_quantize_fp8": (c_int, [FP, c_int, c_int64, c_int, FP, c_int64, FP, c_int64, c_int64, c_void_p]),
+    "nfe_fp8_weight_bytes": (c_uint64, [c_int, c_int]),
+    "nfe_fp8_weight_quantize": (c_int, [FP, c_int, c_int, c_int, c_float, FP, FP, c_void_p]),
+    "nfe_fp8_weight_pack": (c_int, [FP, c_int, c_int, FP, c_void_p]),
+    "nfe_fp8_matmul": (c_int, [POINTER(Fp8MatmulArgs), c_void_p]),
     "nfe_point_query": (c_int, [FP, FP, c_int, c_int, c_int64, FP, FP, FP, FP, FP, c_int, FP, c_int, c_int, c_float,
                                 FP, FP, FP, c_float, c_uint64, FP, c_void_p]),
 }

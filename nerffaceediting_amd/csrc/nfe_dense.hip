@@ -7,6 +7,7 @@
 #include <algorithm>
 #include "nfe_common.h"
 #include "nfe_dense.h"
+#include "nfe_fp8.h"
 
 namespace nfe {
 

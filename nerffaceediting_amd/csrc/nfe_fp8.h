@@ -1,0 +1,473 @@
+// 8-bit dense operators (e4m3 values, one fp32 scale for every block of 128): RMS norm / quantisation of rows, packing of weights and the
+// product of the two.  Part of nfe_dense.hip's code object, beside the fp32 fully-connected layers they are the 8-bit form of.
+#pragma once
+#include "nfe_dense.h"
+#include "nfe_wave.h"
+
+NFE_NO_PACKED_FP32_BEGIN
+namespace nfe {
+namespace fp8 {
+
+constexpr int BLOCK = 128;
+constexpr float E4M3_MAX = 448.0f;
+constexpr float SMALLEST = 1e-30f;       // lower bound of a block's maximum: an all-zero block gets a finite scale and zeros
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+template <int TYPE> struct Elem;
+template <> struct Elem<NFE_F32> { typedef float T; };
+template <> struct Elem<NFE_BF16> { typedef __bf16 T; };
+template <> struct Elem<NFE_F16> { typedef _Float16 T; };
+template <typename T, int N> struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Vec { T e[N]; };
+
+__device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
+__device__ __forceinline__ unsigned abs_bits(float v) { return bits_of(v) & 0x7fffffffu; }     // ordered as |v|, NaN above infinity
+// four values -> four e4m3 bytes, round to nearest even
+__device__ __forceinline__ unsigned e4m3x4(float a, float b, float c, float d) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+
+// ------------------------------------------------------------------------------------------------
+// h = x + residual;  y = h * rsqrt(mean(h^2) + eps) * weight  (NORM) or y = h;  then per 128 columns
+//   a = max(max |y|, 1e-30),  scale = a / 448,  q = e4m3(y / scale)
+// Everything between the load of x and the rounding to e4m3 (and of h to x's type) is fp32.  The maximum is taken on the bits, so a NaN or
+// an infinity in a block makes its scale NaN or infinite and every value of the block reads as NaN.
+// One row belongs to WAVES waves; a lane holds 8 neighbouring columns of every step, so 16 lanes share a scale.  STEPS > 0: the row stays
+// in registers and is read once; STEPS = 0: longer rows, read twice.  VEC: 16-byte loads (columns a multiple of 8, pointers aligned).
+// Memory-bound.
+// ------------------------------------------------------------------------------------------------
+struct NormArgs {
+    const void* x; const void* residual; const float* weight; void* h;
+    unsigned char* q; float* scale; long long q_stride, scale_row, scale_block;
+    long long rows; int cols; float eps;
+};
+
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void load8(float (&v)[8], const void* base, long long at, int left) {      // left: columns from here to the row's end
+    typedef typename Elem<TYPE>::T T;
+    const T* p = (const T*)base + at;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+    if (VEC) {
+        if (left > 0) {
+            const Vec<T, 8> r = *(const Vec<T, 8>*)p;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = (float)r.e[k];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < left) v[k] = (float)p[k];
+    }
+}
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void store8(const float (&v)[8], void* base, long long at, int left) {
+    typedef typename Elem<TYPE>::T T;
+    T* p = (T*)base + at;
+    if (VEC) {
+        if (left > 0) {
+            Vec<T, 8> r;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) r.e[k] = (T)v[k];
+            *(Vec<T, 8>*)p = r;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < left) p[k] = (T)v[k];
+    }
+}
+
+template <int TYPE, bool VEC, bool RES>
+__device__ __forceinline__ void load_h(float (&v)[8], const NormArgs& a, long long row, int col) {
+    const long long at = row * a.cols + col;
+    load8<TYPE, VEC>(v, a.x, at, a.cols - col);
+    if (RES) {
+        float r[8];
+        load8<TYPE, VEC>(r, a.residual, at, a.cols - col);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += r[k];
+    }
+}
+
+// every lane of the wave takes part
+template <bool VEC, bool NORM>
+__device__ __forceinline__ void quantise8(float (&v)[8], const NormArgs& a, long long row, int col, float r) {
+    if (NORM) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= r;
+        if (a.weight) {
+            float w[8];
+            load8<NFE_F32, VEC>(w, a.weight, col, a.cols - col);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= w[k];
+        }
+    }
+    unsigned m = bits_of(SMALLEST);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = umax(m, abs_bits(v[k]));
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) m = umax(m, wave_xor(m, off));
+    const float scale = float_of(m) / E4M3_MAX;
+    const float inv = 1.0f / scale;
+    if (col < a.q_stride) {
+        uint2 w;
+        w.x = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+        w.y = e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+        if (col < (a.cols + BLOCK - 1) / BLOCK * BLOCK) {
+            *(uint2*)(a.q + row * a.q_stride + col) = w;
+            if (((col >> 3) & 15) == 0) a.scale[row * a.scale_row + (long long)(col / BLOCK) * a.scale_block] = scale;
+        }
+    }
+}
+
+template <int TYPE, bool VEC, bool NORM, bool RES, int WAVES, int STEPS>
+__global__ __launch_bounds__(256) void norm_fp8_kernel(NormArgs a) {
+    __shared__ float part[4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const long long row = WAVES == 1 ? (long long)blockIdx.x * 4 + wave : (long long)blockIdx.x;
+    if (row >= a.rows) return;                                        // WAVES == 1 only: no barrier below then
+    const int first = (WAVES == 1 ? 0 : wave * 512) + lane * 8;
+    constexpr int STRIDE = WAVES * 512, KEEP = STEPS > 0 ? STEPS : 1;
+    float v[KEEP][8], sum = 0.0f;
+    if (STEPS > 0) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) load_h<TYPE, VEC, RES>(v[s], a, row, first + s * STRIDE);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            if (RES) store8<TYPE, VEC>(v[s], a.h, row * a.cols + first + s * STRIDE, a.cols - (first + s * STRIDE));
+            if (NORM)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum = fmaf(v[s][k], v[s][k], sum);
+        }
+    } else if (NORM || RES) {
+        for (int col = first; col < a.cols; col += STRIDE) {
+            load_h<TYPE, VEC, RES>(v[0], a, row, col);
+            if (NORM)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum = fmaf(v[0][k], v[0][k], sum);
+        }
+    }
+    float r = 1.0f;
+    if (NORM) {
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) sum += wave_xor(sum, off);
+        if (WAVES > 1) {
+            if (lane == 0) part[wave] = sum;
+            block_sync();
+            sum = (part[0] + part[1]) + (part[2] + part[3]);
+        }
+        r = __builtin_amdgcn_rsqf(sum / (float)a.cols + a.eps);
+    }
+    if (STEPS > 0) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) quantise8<VEC, NORM>(v[s], a, row, first + s * STRIDE, r);
+    } else {
+        const int width = (a.cols + STRIDE - 1) / STRIDE * STRIDE;    // whole waves: quantise8 exchanges between lanes
+        for (int col = first; col < width; col += STRIDE) {
+            load_h<TYPE, VEC, RES>(v[0], a, row, col);
+            if (RES) store8<TYPE, VEC>(v[0], a.h, row * a.cols + col, a.cols - col);
+            quantise8<VEC, NORM>(v[0], a, row, col, r);
+        }
+    }
+}
+
+template <int TYPE, bool VEC, bool NORM, bool RES>
+static void norm_launch(const NormArgs& a, hipStream_t st) {
+    const dim3 narrow((unsigned)((a.rows + 3) / 4)), wide((unsigned)a.rows), b(256);
+    // a wave for a row of up to 2048 columns, four waves for a longer one
+    if (a.cols <= 512) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, VEC, NORM, RES, 1, 1>), narrow, b, 0, st, a);
+    else if (a.cols <= 1024) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, VEC, NORM, RES, 1, 2>), narrow, b, 0, st, a);
+    else if (a.cols <= 2048) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, VEC, NORM, RES, 1, 4>), narrow, b, 0, st, a);
+    else if (a.cols <= 4096) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, VEC, NORM, RES, 4, 2>), wide, b, 0, st, a);
+    else if (a.cols <= 8192) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, VEC, NORM, RES, 4, 4>), wide, b, 0, st, a);
+    else hipLaunchKernelGGL((norm_fp8_kernel<TYPE, VEC, NORM, RES, 4, 0>), wide, b, 0, st, a);
+}
+template <int TYPE>
+static void norm_dispatch(const NormArgs& a, bool norm, hipStream_t st) {
+    const uintptr_t all = (uintptr_t)a.x | (uintptr_t)a.residual | (uintptr_t)a.weight | (uintptr_t)a.h;
+    const bool vec = a.cols % 8 == 0 && all % 16 == 0;
+    if (!norm) {
+        if (vec) norm_launch<TYPE, true, false, false>(a, st); else norm_launch<TYPE, false, false, false>(a, st);
+    } else if (a.residual) {
+        if (vec) norm_launch<TYPE, true, true, true>(a, st); else norm_launch<TYPE, false, true, true>(a, st);
+    } else {
+        if (vec) norm_launch<TYPE, true, true, false>(a, st); else norm_launch<TYPE, false, true, false>(a, st);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Weights [n, k] -> the operand image of v_mfma_f32_16x16x128_f8f6f4: [n/16][k/128][half 2][lane 64][16 bytes], lane l of half h holds
+// columns 64 h + 16 (l / 16) .. + 15 of row l % 16, so a fragment is two contiguous kilobytes.  (The instruction sums over all 128
+// columns, whose order is free as long as both operands share it.)  Rows and columns beyond n and k are zero.
+// ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ long long packed_at(int n, int k, int kblocks) {
+    const int c = k & 127;
+    return ((((long long)(n >> 4) * kblocks + (k >> 7)) * 2 + (c >> 6)) * 64 + ((c >> 4) & 3) * 16 + (n & 15)) * 16 + (c & 15);
+}
+
+// one workgroup per 128 x 128 block; w null: q holds e4m3 bytes already
+template <int TYPE>
+__global__ __launch_bounds__(256) void weight_fp8_kernel(const void* w, const unsigned char* __restrict__ q, int n, int k, float gain,
+                                                         unsigned char* __restrict__ packed, float* __restrict__ scale) {
+    typedef typename Elem<TYPE>::T T;
+    __shared__ unsigned part[4];
+    const int kblocks = gridDim.x, n0 = blockIdx.y * BLOCK, k0 = blockIdx.x * BLOCK;
+    const int c = threadIdx.x & 127, r0 = threadIdx.x >> 7;
+    const T* src = (const T*)w;
+    const int rows = (n + 15) / 16 * 16;
+    float inv = 1.0f;
+    if (w) {
+        unsigned m = bits_of(SMALLEST);
+        for (int r = r0; r < BLOCK; r += 2)
+            if (n0 + r < n)
+                if (k0 + c < k) m = umax(m, abs_bits((float)src[(long long)(n0 + r) * k + k0 + c]));
+        for (int off = 1; off < 64; off <<= 1) m = umax(m, wave_xor(m, off));
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+        block_sync();
+        m = umax(umax(part[0], part[1]), umax(part[2], part[3]));
+        const float s = float_of(m) / E4M3_MAX;
+        if (threadIdx.x == 0) scale[(long long)blockIdx.y * kblocks + blockIdx.x] = s * gain;
+        inv = 1.0f / s;
+    }
+    for (int r = r0; r < BLOCK; r += 2) {
+        if (n0 + r >= rows) break;
+        unsigned byte = 0;
+        if (n0 + r < n)
+            if (k0 + c < k) {
+                const long long at = (long long)(n0 + r) * k + k0 + c;
+                byte = w ? e4m3x4((float)src[at] * inv, 0.0f, 0.0f, 0.0f) & 255u : (unsigned)q[at];
+            }
+        packed[packed_at(n0 + r, k0 + c, kblocks)] = (unsigned char)byte;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// out[m, n] = act( sum_kb a_scale[m, kb] w_scale[n / 128, kb] * (sum over the 128 columns of a[m, .] w[n, .]) + bias_gain bias[n] )
+// A block's sum is scaled and added in fp32, and the result is rounded once, to the output's type.  The block's own sum:
+//   FP8 (bf16 and fp16 outputs): one v_mfma_f32_16x16x128_f8f6f4.  The unit adds eight products at a time in fixed point, at 2^-13 of the
+//     power of two of the largest (measured: next to one product of 2^16, products below 2^3 vanish if they are among its eight and count
+//     to 2^-7 otherwise; truncated towards zero), so a sum is off by less than 7 2^-13 sum|products| - 1.5e-5 of its size for normally
+//     distributed values, an eighth of the rounding to fp16 and a hundredth of that to bf16;
+//   WIDE (fp32 output): both operands widened to bf16, which holds every e4m3 value, and four v_mfma_f32_16x16x32_bf16: exact products,
+//     fp32 sums, half the rate.
+// The weights are the instruction's first operand: lane l then holds outputs 4 (l / 16) .. + 3 of row l % 16, whose scale is one number
+// per lane.
+// ------------------------------------------------------------------------------------------------
+struct MatmulArgs {
+    const unsigned char* a; const float* a_scale; const unsigned char* w; const float* w_scale; const float* bias; void* out;
+    long long a_stride, scale_row, scale_block;
+    int m, n, kblocks, lrelu, out_type, vec_out; float bias_gain;
+};
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ bf16x8 widen8(int lo, int hi) {
+    union { bf16x2 p[4]; bf16x8 v; } u;
+    u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+    u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+    u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+    u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+    return u.v;
+}
+// A fragment: the 32 values of 128 columns that a lane holds, in the form the instruction takes
+template <bool WIDE> struct Frag;
+template <> struct Frag<false> {
+    i32x8 v;
+    __device__ __forceinline__ void set(const i32x4& lo, const i32x4& hi) { v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
+};
+template <> struct Frag<true> {
+    bf16x8 v[4];
+    __device__ __forceinline__ void set(const i32x4& lo, const i32x4& hi) {
+        v[0] = widen8(lo[0], lo[1]); v[1] = widen8(lo[2], lo[3]); v[2] = widen8(hi[0], hi[1]); v[3] = widen8(hi[2], hi[3]);
+    }
+};
+__device__ __forceinline__ f32x4 mfma_block(const Frag<false>& w, const Frag<false>& a) {
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, a.v, zero, 0, 0, 0, 0, 0, 0);      // scales 0: the unscaled instruction
+}
+__device__ __forceinline__ f32x4 mfma_block(const Frag<true>& w, const Frag<true>& a) {
+    f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], a.v[i], d, 0, 0, 0);
+    return d;
+}
+
+template <int TYPE>
+__device__ __forceinline__ void store4(const float (&v)[4], void* out, long long at, int left, int vec) {
+    typedef typename Elem<TYPE>::T T;
+    T* p = (T*)out + at;
+    if (vec) {                                    // the row length is a multiple of 4: all four columns are inside
+        Vec<T, 4> r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.e[i] = (T)v[i];
+        *(Vec<T, 4>*)p = r;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < left) p[i] = (T)v[i];
+    }
+}
+// columns n .. n + 3 of row m
+__device__ __forceinline__ void finish4(const MatmulArgs& A, f32x4 s, int m, int n) {
+    if (m >= A.m) return;
+    if (n >= A.n) return;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = s[i];
+        if (A.bias) v[i] = fmaf(A.bias[n + i < A.n ? n + i : A.n - 1], A.bias_gain, v[i]);
+    }
+    if (A.lrelu)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (v[i] < 0.0f ? v[i] * 0.2f : v[i]) * 1.4142135623730951f;      // bias_act 'lrelu': alpha 0.2, gain sqrt(2)
+    const long long at = (long long)m * A.n + n;
+    if (A.out_type == NFE_F32) store4<NFE_F32>(v, A.out, at, A.n - n, A.vec_out);
+    else if (A.out_type == NFE_BF16) store4<NFE_BF16>(v, A.out, at, A.n - n, A.vec_out);
+    else store4<NFE_F16>(v, A.out, at, A.n - n, A.vec_out);
+}
+
+// Few rows.  A workgroup of WAVES waves owns 16 columns of the output and 16 MT rows; the waves share the K blocks, read both operands
+// straight into registers and join their sums through LDS.  Every weight is read once: bound by that.
+template <bool WIDE, int MT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void matmul_rows_kernel(MatmulArgs A) {
+    __shared__ f32x4 part[WAVES][MT][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int nt = blockIdx.x, m0 = blockIdx.y * (16 * MT);
+    const int g = lane >> 4, r = lane & 15;
+    const unsigned char* wp = A.w + (long long)nt * A.kblocks * 2048 + lane * 16;
+    const unsigned char* ap[MT]; const float* sp[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int m = m0 + 16 * t + r;
+        const long long row = m < A.m ? m : A.m - 1;
+        ap[t] = A.a + row * A.a_stride + g * 16;
+        sp[t] = A.a_scale + row * A.scale_row;
+    }
+    const float* ws = A.w_scale + (long long)(nt >> 3) * A.kblocks;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int kb = wave; kb < A.kblocks; kb += WAVES) {
+        Frag<WIDE> w;
+        w.set(*(const i32x4*)(wp + (long long)kb * 2048), *(const i32x4*)(wp + (long long)kb * 2048 + 1024));
+        const float sw = ws[kb];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            Frag<WIDE> a;
+            a.set(*(const i32x4*)(ap[t] + (long long)kb * 128), *(const i32x4*)(ap[t] + (long long)kb * 128 + 64));
+            const float s = sp[t][kb * A.scale_block] * sw;
+            const f32x4 d = mfma_block(w, a);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(d[i], s, acc[t][i]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+    block_sync();
+    for (int e = threadIdx.x; e < MT * 64; e += 64 * WAVES) {
+        const int t = e >> 6, l = e & 63;
+        f32x4 s = part[0][t][l];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) s += part[w][t][l];
+        finish4(A, s, m0 + 16 * t + (l & 15), nt * 16 + (l >> 4) * 4);
+    }
+}
+
+template <bool WIDE>
+static int matmul_launch(const MatmulArgs& A, hipStream_t st) {
+    const unsigned nt = (unsigned)((A.n + 15) / 16);
+    const long long mt = ((long long)A.m + 63) / 64;
+    if (A.m <= 16) hipLaunchKernelGGL((matmul_rows_kernel<WIDE, 1, 8>), dim3(nt), dim3(512), 0, st, A);
+    else if (A.m <= 32) hipLaunchKernelGGL((matmul_rows_kernel<WIDE, 2, 8>), dim3(nt), dim3(512), 0, st, A);
+    else {
+        NFE_REQUIRE(mt <= 65535, "nfe_fp8_matmul: m=%d is too large", A.m);
+        hipLaunchKernelGGL((matmul_rows_kernel<WIDE, 4, 8>), dim3(nt, (unsigned)mt), dim3(512), 0, st, A);
+    }
+    return NFE_OK;
+}
+
+static int check_rows(const char* who, long long rows, int cols) {
+    NFE_REQUIRE(rows > 0 && rows <= 0x7fffffffll, "%s: rows=%lld must be in [1, 2^31)", who, rows);
+    NFE_REQUIRE(cols > 0 && cols <= (1 << 30), "%s: cols=%d must be in [1, 2^30]", who, cols);
+    return NFE_OK;
+}
+static int norm_entry(const char* who, NormArgs& a, int dtype, bool norm, nfe_stream_t stream) {
+    if (int rc = check_rows(who, a.rows, a.cols)) return rc;
+    NFE_REQUIRE(dtype == NFE_F32 || dtype == NFE_BF16 || dtype == NFE_F16, "%s: unknown dtype %d", who, dtype);
+    NFE_REQUIRE(a.x && a.q && a.scale, "%s: null pointer", who);
+    NFE_REQUIRE((a.residual != nullptr) == (a.h != nullptr), "%s: residual and h come in pairs", who);
+    const int width = (a.cols + BLOCK - 1) / BLOCK * BLOCK;
+    NFE_REQUIRE(a.q_stride >= width && a.q_stride % 8 == 0 && (uintptr_t)a.q % 8 == 0, "%s: q rows must be 8-byte aligned and at least %d bytes apart", who, width);
+    NFE_REQUIRE(!norm || a.eps > 0.0f, "%s: eps must be positive", who);
+    if (dtype == NFE_F32) norm_dispatch<NFE_F32>(a, norm, (hipStream_t)stream);
+    else if (dtype == NFE_BF16) norm_dispatch<NFE_BF16>(a, norm, (hipStream_t)stream);
+    else norm_dispatch<NFE_F16>(a, norm, (hipStream_t)stream);
+    NFE_CHECK_LAUNCH(who);
+    return NFE_OK;
+}
+static int check_weight(const char* who, int n, int k) {
+    NFE_REQUIRE(n > 0 && k > 0 && n <= (1 << 23) && k <= (1 << 30), "%s: bad sizes n=%d k=%d", who, n, k);
+    return NFE_OK;
+}
+
+}  // namespace fp8
+}  // namespace nfe
+NFE_NO_PACKED_FP32_END
+
+extern "C" int nfe_rms_norm_fp8(const void* x, const void* residual, const float* weight, int dtype, int64_t rows, int cols, float eps, void* h, void* q,
+                                int64_t q_stride, float* scale, int64_t scale_row_stride, int64_t scale_block_stride, nfe_stream_t stream) {
+    nfe::fp8::NormArgs a{x, residual, weight, h, (unsigned char*)q, scale, q_stride, scale_row_stride, scale_block_stride, rows, cols, eps};
+    return nfe::fp8::norm_entry("nfe_rms_norm_fp8", a, dtype, true, stream);
+}
+extern "C" int nfe_quantize_fp8(const void* x, int dtype, int64_t rows, int cols, void* q, int64_t q_stride, float* scale, int64_t scale_row_stride,
+                                int64_t scale_block_stride, nfe_stream_t stream) {
+    nfe::fp8::NormArgs a{x, nullptr, nullptr, nullptr, (unsigned char*)q, scale, q_stride, scale_row_stride, scale_block_stride, rows, cols, 0.0f};
+    return nfe::fp8::norm_entry("nfe_quantize_fp8", a, dtype, false, stream);
+}
+extern "C" uint64_t nfe_fp8_weight_bytes(int n, int k) {
+    return n > 0 && k > 0 ? ((uint64_t)n + 15) / 16 * (((uint64_t)k + 127) / 128) * 2048 : 0;
+}
+extern "C" int nfe_fp8_weight_quantize(const void* w, int dtype, int n, int k, float gain, void* packed, float* scale, nfe_stream_t stream) {
+    using namespace nfe::fp8;
+    if (int rc = check_weight("nfe_fp8_weight_quantize", n, k)) return rc;
+    NFE_REQUIRE(w && packed && scale, "nfe_fp8_weight_quantize: null pointer");
+    NFE_REQUIRE(dtype == NFE_F32 || dtype == NFE_BF16 || dtype == NFE_F16, "nfe_fp8_weight_quantize: unknown dtype %d", dtype);
+    const dim3 grid((unsigned)((k + BLOCK - 1) / BLOCK), (unsigned)((n + BLOCK - 1) / BLOCK));
+    auto kernel = dtype == NFE_F32 ? weight_fp8_kernel<NFE_F32> : dtype == NFE_BF16 ? weight_fp8_kernel<NFE_BF16> : weight_fp8_kernel<NFE_F16>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, w, (const unsigned char*)nullptr, n, k, gain, (unsigned char*)packed, scale);
+    NFE_CHECK_LAUNCH("nfe_fp8_weight_quantize");
+    return NFE_OK;
+}
+extern "C" int nfe_fp8_weight_pack(const void* q, int n, int k, void* packed, nfe_stream_t stream) {
+    using namespace nfe::fp8;
+    if (int rc = check_weight("nfe_fp8_weight_pack", n, k)) return rc;
+    NFE_REQUIRE(q && packed, "nfe_fp8_weight_pack: null pointer");
+    const dim3 grid((unsigned)((k + BLOCK - 1) / BLOCK), (unsigned)((n + BLOCK - 1) / BLOCK));
+    hipLaunchKernelGGL(weight_fp8_kernel<NFE_F32>, grid, dim3(256), 0, (hipStream_t)stream, (const void*)nullptr, (const unsigned char*)q, n, k, 1.0f,
+                       (unsigned char*)packed, (float*)nullptr);
+    NFE_CHECK_LAUNCH("nfe_fp8_weight_pack");
+    return NFE_OK;
+}
+extern "C" int nfe_fp8_matmul(const nfe_fp8_matmul_args* p, nfe_stream_t stream) {
+    using namespace nfe::fp8;
+    NFE_REQUIRE(p, "nfe_fp8_matmul: args is null");
+    NFE_REQUIRE(p->struct_size == sizeof(*p), "nfe_fp8_matmul: struct_size %u != %zu", p->struct_size, sizeof(*p));
+    NFE_REQUIRE(p->q && p->scale && p->packed && p->w_scale && p->out, "nfe_fp8_matmul: null pointer");
+    if (int rc = check_weight("nfe_fp8_matmul", p->n, p->k)) return rc;
+    NFE_REQUIRE(p->m > 0 && p->m <= (1 << 30), "nfe_fp8_matmul: m=%d must be in [1, 2^30]", p->m);
+    const int kblocks = (p->k + BLOCK - 1) / BLOCK;
+    NFE_REQUIRE(p->q_stride >= (int64_t)kblocks * BLOCK && p->q_stride % 16 == 0 && (uintptr_t)p->q % 16 == 0 && (uintptr_t)p->packed % 16 == 0,
+                "nfe_fp8_matmul: q rows must be 16-byte aligned and at least %d bytes apart", kblocks * BLOCK);
+    NFE_REQUIRE(p->out_dtype == NFE_F32 || p->out_dtype == NFE_BF16 || p->out_dtype == NFE_F16, "nfe_fp8_matmul: unknown out_dtype %d", p->out_dtype);
+    const int size = p->out_dtype == NFE_F32 ? 4 : 2;
+    NFE_REQUIRE((uintptr_t)p->out % size == 0, "nfe_fp8_matmul: misaligned out");
+    MatmulArgs A{(const unsigned char*)p->q, p->scale, (const unsigned char*)p->packed, p->w_scale, p->bias, p->out, p->q_stride, p->scale_row_stride,
+                 p->scale_block_stride, p->m, p->n, kblocks, p->lrelu, p->out_dtype, p->n % 4 == 0 && (uintptr_t)p->out % (4 * size) == 0, p->bias_gain};
+    if (int rc = p->out_dtype == NFE_F32 ? matmul_launch<true>(A, (hipStream_t)stream) : matmul_launch<false>(A, (hipStream_t)stream)) return rc;
+    NFE_CHECK_LAUNCH("nfe_fp8_matmul");
+    return NFE_OK;
+}

@@ -54,15 +54,26 @@ class FullyConnectedLayer(torch.nn.Module):
         return dense_ops.fully_connected(x, self.weight.detach(), None if self.bias is None else self.bias.detach(),
                                          self.weight_gain, self.bias_gain, self.activation == "lrelu", out, out_offset)
 
+    def forward_fp8(self, q, scale):
+        """forward() on 8-bit rows (dense_ops.rms_norm_fp8 / quantize_fp8) and this layer's weights rounded to e4m3 -> fp32."""
+        key = (self.weight.data_ptr(), self.weight._version, tuple(self.weight.shape))
+        if getattr(self, "_fp8_key", None) != key:
+            self._fp8 = dense_ops.fp8_weight(self.weight.detach(), gain=self.weight_gain)
+            _publish()
+            self._fp8_key = key
+        return dense_ops.fp8_matmul(q, scale, self._fp8, None if self.bias is None else self.bias.detach(), self.bias_gain, self.activation == "lrelu")
+
     def extra_repr(self):
         return f"in_features={self.in_features:d}, out_features={self.out_features:d}, activation={self.activation:s}"
 
 
 class MappingNetwork(torch.nn.Module):
-    """networks_stylegan2.py:193-271."""
+    """networks_stylegan2.py:193-271.  fc_math='fp8' runs the fully-connected stack on e4m3 operands (one scale for every 128 input
+    features of a row and every 128 x 128 block of a weight, fp32 sums): for large batches of latents; w differs from the fp32 path's by
+    the operands' rounding (about 3 % of its own size)."""
 
     def __init__(self, z_dim, c_dim, w_dim, num_ws, num_layers=8, embed_features=None, layer_features=None,
-                 activation="lrelu", lr_multiplier=0.01, w_avg_beta=0.998):
+                 activation="lrelu", lr_multiplier=0.01, w_avg_beta=0.998, fc_math=None):
         super().__init__()
         self.z_dim, self.c_dim, self.w_dim, self.num_ws = z_dim, c_dim, w_dim, num_ws
         self.num_layers, self.w_avg_beta = num_layers, w_avg_beta
@@ -70,6 +81,11 @@ class MappingNetwork(torch.nn.Module):
             embed_features = w_dim
         if c_dim == 0:
             embed_features = 0
+        if fc_math not in (None, "fp8"):
+            raise ValueError(f"unknown fc_math {fc_math!r}")
+        if fc_math == "fp8" and (z_dim % dense_ops.FP8_BLOCK or embed_features % dense_ops.FP8_BLOCK):
+            raise ValueError(f"fc_math='fp8' needs z_dim ({z_dim}) and embed_features ({embed_features}) in multiples of {dense_ops.FP8_BLOCK}")
+        self.fc_math = fc_math
         if layer_features is None:
             layer_features = w_dim
         features_list = [z_dim + embed_features] + [layer_features] * (num_layers - 1) + [w_dim]
@@ -87,6 +103,11 @@ class MappingNetwork(torch.nn.Module):
         assert self.z_dim > 0 and self.num_ws is not None
         assert z.shape[1] == self.z_dim, f"Wrong size for dimension 1: got {z.shape[1]}, expected {self.z_dim}"   # misc.assert_shape
         N = z.shape[0]
+        psi = float(truncation_psi)
+        cutoff = self.num_ws if truncation_cutoff is None else min(int(truncation_cutoff), self.num_ws)
+        if self.fc_math == "fp8":
+            x = self._layers_fp8(z.detach().to(torch.float32), c)
+            return dense_ops.broadcast_truncate(x, self.w_avg if psi != 1 else None, self.num_ws, psi, cutoff)
         buf = torch.empty(N, self.z_dim + self.embed_features, device=z.device)
         dense_ops.normalize_2nd_moment(z.to(torch.float32), out=buf, out_offset=0)                 # :240
         if self.c_dim > 0:
@@ -96,9 +117,22 @@ class MappingNetwork(torch.nn.Module):
         x = buf
         for idx in range(self.num_layers):
             x = getattr(self, f"fc{idx}")(x)
-        psi = float(truncation_psi)
-        cutoff = self.num_ws if truncation_cutoff is None else min(int(truncation_cutoff), self.num_ws)
         return dense_ops.broadcast_truncate(x, self.w_avg if psi != 1 else None, self.num_ws, psi, cutoff)   # :257-267
+
+    def _layers_fp8(self, z, c):
+        """The norms (:240, :244) and the layers on 8-bit operands; the camera's embedding (25 inputs) stays fp32."""
+        N, width = z.shape[0], self.z_dim + self.embed_features
+        q = torch.empty(N, width, dtype=torch.float8_e4m3fn, device=z.device)
+        scale = torch.empty(width // dense_ops.FP8_BLOCK, N, device=z.device).t()
+        dense_ops.rms_norm_fp8(z, out=(q, scale))
+        if self.c_dim > 0:
+            assert c.shape[1] == self.c_dim, f"Wrong size for dimension 1: got {c.shape[1]}, expected {self.c_dim}"
+            dense_ops.rms_norm_fp8(self.embed(c.detach().to(torch.float32)), out=(q, scale), out_offset=self.z_dim)
+        for idx in range(self.num_layers):
+            x = getattr(self, f"fc{idx}").forward_fp8(q, scale)
+            if idx + 1 < self.num_layers:
+                q, scale = dense_ops.quantize_fp8(x)
+        return x
 
 
 class SynthesisLayer(torch.nn.Module):
