@@ -377,16 +377,149 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_rows_kernel(MatmulArgs A) {
     }
 }
 
+// Many rows.  A workgroup of WM x WN waves owns (16 MT WM) rows x (16 NT WN) columns; per 128 columns of K
+//   * the rows' values come into LDS by LDS-DMA, one K block ahead: [row][8 chunks of 16 bytes], chunk c of row r at c ^ (r & 7) - the
+//     DMA's destination is linear, so the permutation is applied to its source - which makes the fragment reads free of bank conflicts;
+//     their scales beside them;
+//   * the weights' fragments, already in operand order, go straight from L2 to registers, one K block ahead: through LDS they would take it
+//     beyond its bandwidth;
+//   * a wave multiplies its MT x NT fragments: MT + NT reads for MT NT matrix instructions.
+// Every load of a K block is in flight while the block before it is multiplied; one barrier a block.
+// Workgroups b, b + 8, .. run on one XCD: each XCD gets a contiguous range of tiles, GROUP row tiles deep, so that its L2 serves both operands.
+// LDS-DMA: 64 lanes x 16 (4) bytes from base + offset into 1 KiB (256 bytes) at dst.  Inline assembly, because the compiler would wait for the DMA
+// into the next buffer before the reads of this one; the waits are explicit (buffer_wait).
+__device__ __forceinline__ void dma16(const void* base, unsigned offset, const void* dst) {
+    const unsigned l = (unsigned)(unsigned long long)(__attribute__((address_space(3))) const void*)dst;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(l), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(const void* base, unsigned offset, const void* dst) {
+    const unsigned l = (unsigned)(unsigned long long)(__attribute__((address_space(3))) const void*)dst;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(l), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void buffer_wait() {          // own loads have landed, then everybody's
+    __builtin_amdgcn_s_waitcnt(0x0F70);                  // vmcnt(0), and nothing else; the builtin, so that the compiler counts its own loads as landed too
+    block_sync();
+}
+
+constexpr int GROUP = 4;
+// tile of workgroup b: bijective for any number of tiles
+__device__ __forceinline__ void tile_of(int b, int tm, int tn, int& im, int& in) {
+    const int total = tm * tn, q = total / 8, r = total % 8, x = b & 7, i = b >> 3;
+    const int t = x * q + (x < r ? x : r) + i;
+    const int per = GROUP * tn, g = t / per, rest = t - g * per;
+    const int depth = tm - g * GROUP < GROUP ? tm - g * GROUP : GROUP;
+    in = rest / depth;
+    im = g * GROUP + rest - in * depth;
+}
+
+template <bool WIDE, int WM, int WN, int MT, int NT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs A, int tm, int tn) {
+    constexpr int THREADS = 64 * WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
+    constexpr int LOADS = BM * 8 / THREADS;              // DMA instructions a wave issues for a block of rows
+    static_assert(BM * 8 % THREADS == 0 && BM % 64 == 0 && BM / 64 <= WM * WN && 128 % (16 * NT) == 0, "tile shape");
+    __shared__ __attribute__((aligned(16))) unsigned char rows[2][BM * 128];
+    __shared__ __attribute__((aligned(16))) float scales[2][BM];
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
+    int im, in;
+    tile_of((int)blockIdx.x, tm, tn, im, in);
+    const int m0 = im * BM, n0 = in * BN + wn * (16 * NT);
+
+    const unsigned char* a_base = A.a + (long long)m0 * A.a_stride;
+    unsigned a_off[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int c = i * THREADS + tid, row = c >> 3;
+        const int inside = m0 + row < A.m ? row : A.m - 1 - m0;
+        a_off[i] = (unsigned)inside * (unsigned)A.a_stride + (unsigned)(((c & 7) ^ (row & 7)) * 16);
+    }
+    const int srow = wave * 64 + lane;
+    const float* s_base = A.a_scale + (long long)m0 * A.scale_row;
+    const unsigned s_off = (unsigned)(m0 + srow < A.m ? srow : A.m - 1 - m0) * (unsigned)A.scale_row * 4u;
+    const int last = (A.n + 15) / 16 - 1;
+    const unsigned char* w_base[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int nt = n0 / 16 + j < last ? n0 / 16 + j : last;
+        w_base[j] = A.w + (long long)nt * A.kblocks * 2048;
+    }
+    const int nb = n0 / BLOCK < (A.n - 1) / BLOCK ? n0 / BLOCK : (A.n - 1) / BLOCK;
+    const float* w_scale = A.w_scale + (long long)nb * A.kblocks;
+
+    auto fetch_rows = [&](int kb, int buf) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) dma16(a_base + (long long)kb * 128, a_off[i], &rows[buf][(i * THREADS + wave * 64) * 16]);
+        if (wave < BM / 64) dma4(s_base + kb * A.scale_block, s_off, &scales[buf][wave * 64]);
+    };
+    i32x4 w_next[NT][2];
+    auto fetch_weights = [&](int kb) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w_next[j][h] = *(const i32x4*)(w_base[j] + (long long)kb * 2048 + h * 1024 + lane * 16);
+    };
+
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int at = (wm * MT * 16 + r) * 128, at0 = at + ((g ^ (r & 7)) * 16), at1 = at + (((g + 4) ^ (r & 7)) * 16);
+    fetch_rows(0, 0);
+    fetch_weights(0);
+    buffer_wait();
+    for (int kb = 0; kb < A.kblocks; ++kb) {
+        const int buf = kb & 1;
+        Frag<WIDE> w[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) w[j].set(w_next[j][0], w_next[j][1]);
+        const float sw = w_scale[kb];
+        if (kb + 1 < A.kblocks) {
+            fetch_rows(kb + 1, buf ^ 1);
+            fetch_weights(kb + 1);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            Frag<WIDE> a;
+            a.set(*(const i32x4*)&rows[buf][at0 + i * 2048], *(const i32x4*)&rows[buf][at1 + i * 2048]);
+            const float s = scales[buf][wm * MT * 16 + i * 16 + r] * sw;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const f32x4 d = mfma_block(w[j], a);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(d[k], s, acc[i][j][k]);
+            }
+        }
+        buffer_wait();
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) finish4(A, acc[i][j], m0 + (wm * MT + i) * 16 + r, n0 + 16 * j + 4 * g);
+}
+
+template <bool WIDE, int WM, int WN, int MT, int NT>
+static int tile_launch(const MatmulArgs& A, hipStream_t st) {
+    constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN;
+    const long long tm = ((long long)A.m + BM - 1) / BM, tn = ((long long)A.n + BN - 1) / BN;
+    NFE_REQUIRE(tm * tn <= 0x7fffffffll, "nfe_fp8_matmul: m=%d n=%d are too large", A.m, A.n);
+    hipLaunchKernelGGL((matmul_tile_kernel<WIDE, WM, WN, MT, NT>), dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), 0, st, A, (int)tm, (int)tn);
+    return NFE_OK;
+}
+
+// Offsets inside a tile are 32-bit: 256 rows of up to 2^23 bytes (and scales that far apart); anything wider stays on the rows kernel.
 template <bool WIDE>
 static int matmul_launch(const MatmulArgs& A, hipStream_t st) {
     const unsigned nt = (unsigned)((A.n + 15) / 16);
     const long long mt = ((long long)A.m + 63) / 64;
+    const bool near = A.a_stride <= (1 << 23) && A.scale_row <= (1 << 21);
     if (A.m <= 16) hipLaunchKernelGGL((matmul_rows_kernel<WIDE, 1, 8>), dim3(nt), dim3(512), 0, st, A);
     else if (A.m <= 32) hipLaunchKernelGGL((matmul_rows_kernel<WIDE, 2, 8>), dim3(nt), dim3(512), 0, st, A);
-    else {
-        NFE_REQUIRE(mt <= 65535, "nfe_fp8_matmul: m=%d is too large", A.m);
+    else if (A.m <= 64 || !near) {
+        NFE_REQUIRE(mt <= 65535, "nfe_fp8_matmul: m=%d is too large for rows %lld bytes apart", A.m, A.a_stride);
         hipLaunchKernelGGL((matmul_rows_kernel<WIDE, 4, 8>), dim3(nt, (unsigned)mt), dim3(512), 0, st, A);
-    }
+    } else if (!WIDE && ((long long)A.m + 255) / 256 * (((long long)A.n + 255) / 256) >= 200) return tile_launch<false, 2, 4, 8, 4>(A, st);
+    else return tile_launch<WIDE, 2, 2, 4, 4>(A, st);
     return NFE_OK;
 }
 
@@ -463,6 +596,7 @@ extern "C" int nfe_fp8_matmul(const nfe_fp8_matmul_args* p, nfe_stream_t stream)
     NFE_REQUIRE(p->q_stride >= (int64_t)kblocks * BLOCK && p->q_stride % 16 == 0 && (uintptr_t)p->q % 16 == 0 && (uintptr_t)p->packed % 16 == 0,
                 "nfe_fp8_matmul: q rows must be 16-byte aligned and at least %d bytes apart", kblocks * BLOCK);
     NFE_REQUIRE(p->out_dtype == NFE_F32 || p->out_dtype == NFE_BF16 || p->out_dtype == NFE_F16, "nfe_fp8_matmul: unknown out_dtype %d", p->out_dtype);
+    NFE_REQUIRE(p->scale_row_stride >= 0 && p->scale_block_stride >= 0, "nfe_fp8_matmul: negative scale stride");
     const int size = p->out_dtype == NFE_F32 ? 4 : 2;
     NFE_REQUIRE((uintptr_t)p->out % size == 0, "nfe_fp8_matmul: misaligned out");
     MatmulArgs A{(const unsigned char*)p->q, p->scale, (const unsigned char*)p->packed, p->w_scale, p->bias, p->out, p->q_stride, p->scale_row_stride,
