@@ -296,6 +296,11 @@ __device__ __forceinline__ f32x4 mfma_block(const Frag<true>& w, const Frag<true
     return d;
 }
 
+// No instruction: what follows and needs `a` comes after what made `acc`.  Without it the compiler issues a block's products first and its
+// additions after them, and spills.
+__device__ __forceinline__ void in_order(f32x4& acc, Frag<false>& a) { asm volatile("" : "+v"(acc), "+v"(a.v)); }
+__device__ __forceinline__ void in_order(f32x4& acc, Frag<true>& a) { asm volatile("" : "+v"(acc), "+v"(a.v[0]), "+v"(a.v[1]), "+v"(a.v[2]), "+v"(a.v[3])); }
+
 template <int TYPE>
 __device__ __forceinline__ void store4(const float (&v)[4], void* out, long long at, int left, int vec) {
     typedef typename Elem<TYPE>::T T;
@@ -378,13 +383,15 @@ __global__ __launch_bounds__(64 * WAVES) void matmul_rows_kernel(MatmulArgs A) {
 }
 
 // Many rows.  A workgroup of WM x WN waves owns (16 MT WM) rows x (16 NT WN) columns; per 128 columns of K
-//   * the rows' values come into LDS by LDS-DMA, one K block ahead: [row][8 chunks of 16 bytes], chunk c of row r at c ^ (r & 7) - the
+//   * the rows' values come into a ring of LDS buffers by LDS-DMA: [row][8 chunks of 16 bytes], chunk c of row r at c ^ (r & 7) - the
 //     DMA's destination is linear, so the permutation is applied to its source - which makes the fragment reads free of bank conflicts;
 //     their scales beside them;
-//   * the weights' fragments, already in operand order, go straight from L2 to registers, one K block ahead: through LDS they would take it
-//     beyond its bandwidth;
-//   * a wave multiplies its MT x NT fragments: MT + NT reads for MT NT matrix instructions.
-// Every load of a K block is in flight while the block before it is multiplied; one barrier a block.
+//   * the weights' fragments, already in operand order, go straight from L2 to registers: through LDS they would take it beyond its bandwidth;
+//   * a wave multiplies its MT x NT fragments, MT + NT reads for MT NT matrix instructions; a product is scaled into its accumulator
+//     LAG instructions after it was issued, so that the vector unit works under the matrix unit.
+// Block kb begins with a wait for every load issued a whole block before (rows of kb + 1, weights of kb) and issues the rows of kb + 2 and the
+// weights of kb + 1.  The one barrier, in the middle of the block, says that the rows of kb + 1 are there for everybody, so no wave stops
+// between blocks; and as nobody is left in block kb - 2 then, buffer (kb + 2) % 4 is free when block kb begins.
 // Workgroups b, b + 8, .. run on one XCD: each XCD gets a contiguous range of tiles, GROUP row tiles deep, so that its L2 serves both operands.
 // LDS-DMA: 64 lanes x 16 (4) bytes from base + offset into 1 KiB (256 bytes) at dst.  Inline assembly, because the compiler would wait for the DMA
 // into the next buffer before the reads of this one; the waits are explicit (buffer_wait).
@@ -396,10 +403,8 @@ __device__ __forceinline__ void dma4(const void* base, unsigned offset, const vo
     const unsigned l = (unsigned)(unsigned long long)(__attribute__((address_space(3))) const void*)dst;
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(l), "v"(offset), "s"(base) : "memory", "m0");
 }
-__device__ __forceinline__ void buffer_wait() {          // own loads have landed, then everybody's
-    __builtin_amdgcn_s_waitcnt(0x0F70);                  // vmcnt(0), and nothing else; the builtin, so that the compiler counts its own loads as landed too
-    block_sync();
-}
+// the builtin, so that the compiler counts its own loads as landed too: vmcnt(0), and nothing else
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); asm volatile("" ::: "memory"); }
 
 constexpr int GROUP = 4;
 // tile of workgroup b: bijective for any number of tiles
@@ -417,8 +422,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs
     constexpr int THREADS = 64 * WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
     constexpr int LOADS = BM * 8 / THREADS;              // DMA instructions a wave issues for a block of rows
     static_assert(BM * 8 % THREADS == 0 && BM % 64 == 0 && BM / 64 <= WM * WN && 128 % (16 * NT) == 0, "tile shape");
-    __shared__ __attribute__((aligned(16))) unsigned char rows[2][BM * 128];
-    __shared__ __attribute__((aligned(16))) float scales[2][BM];
+    __shared__ __attribute__((aligned(16))) unsigned char rows[4][BM * 128];
+    __shared__ __attribute__((aligned(16))) float scales[4][BM];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
     int im, in;
@@ -446,51 +451,88 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs
     const int nb = n0 / BLOCK < (A.n - 1) / BLOCK ? n0 / BLOCK : (A.n - 1) / BLOCK;
     const float* w_scale = A.w_scale + (long long)nb * A.kblocks;
 
-    auto fetch_rows = [&](int kb, int buf) {
+    struct Weights { i32x4 v[NT][2]; float scale; };
+    auto fetch_rows = [&](int kb) {
+        const int buf = kb & 3;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) dma16(a_base + (long long)kb * 128, a_off[i], &rows[buf][(i * THREADS + wave * 64) * 16]);
         if (wave < BM / 64) dma4(s_base + kb * A.scale_block, s_off, &scales[buf][wave * 64]);
     };
-    i32x4 w_next[NT][2];
-    auto fetch_weights = [&](int kb) {
+    auto fetch_weights = [&](Weights& w, int kb) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) w_next[j][h] = *(const i32x4*)(w_base[j] + (long long)kb * 2048 + h * 1024 + lane * 16);
+            for (int h = 0; h < 2; ++h) w.v[j][h] = *(const i32x4*)(w_base[j] + (long long)kb * 2048 + h * 1024 + lane * 16);
+        w.scale = w_scale[kb];
+    };
+    const int at = (wm * MT * 16 + r) * 128, at0 = at + ((g ^ (r & 7)) * 16), at1 = at + (((g + 4) ^ (r & 7)) * 16), st = wm * MT * 16 + r;
+    struct Row { i32x4 lo, hi; float scale; };
+    auto read_row = [&](Row& a, int kb, int i) {
+        const int buf = kb & 3;
+        a.lo = *(const i32x4*)&rows[buf][at0 + i * 2048];
+        a.hi = *(const i32x4*)&rows[buf][at1 + i * 2048];
+        a.scale = scales[buf][st + i * 16];
     };
 
-    f32x4 acc[MT][NT];
+    constexpr int LAG = 2, SLOTS = 4;                    // SLOTS divides MT NT: products keep their slots from block to block
+    static_assert(MT * NT % SLOTS == 0 && MT % 2 == 0 && NT >= LAG, "schedule");
+    f32x4 acc[MT][NT], d[SLOTS];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const int at = (wm * MT * 16 + r) * 128, at0 = at + ((g ^ (r & 7)) * 16), at1 = at + (((g + 4) ^ (r & 7)) * 16);
-    fetch_rows(0, 0);
-    fetch_weights(0);
-    buffer_wait();
-    for (int kb = 0; kb < A.kblocks; ++kb) {
-        const int buf = kb & 1;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) d[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float s_now = 0.0f, s_before = 0.0f;
+    Row row;
+    Weights even, odd;
+
+    auto block = [&](int kb, const Weights& raw, Weights& next) {
+        wait_loads();
+        if (kb + 2 < A.kblocks) fetch_rows(kb + 2);
         Frag<WIDE> w[NT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) w[j].set(w_next[j][0], w_next[j][1]);
-        const float sw = w_scale[kb];
-        if (kb + 1 < A.kblocks) {
-            fetch_rows(kb + 1, buf ^ 1);
-            fetch_weights(kb + 1);
-        }
+        for (int j = 0; j < NT; ++j) w[j].set(raw.v[j][0], raw.v[j][1]);
+        const float sw = raw.scale;
+        if (kb + 1 < A.kblocks) fetch_weights(next, kb + 1);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
+            if (i == MT / 2) block_sync();
             Frag<WIDE> a;
-            a.set(*(const i32x4*)&rows[buf][at0 + i * 2048], *(const i32x4*)&rows[buf][at1 + i * 2048]);
-            const float s = scales[buf][wm * MT * 16 + i * 16 + r] * sw;
+            a.set(row.lo, row.hi);
+            s_before = s_now;
+            s_now = row.scale * sw;
+            if (i + 1 < MT) read_row(row, kb, i + 1);
+            else read_row(row, kb + 1, 0);               // after the last block: whatever the ring holds, unused
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const f32x4 d = mfma_block(w[j], a);
+                const int t = i * NT + j, old = (t + SLOTS - LAG) % SLOTS;
+                d[t % SLOTS] = mfma_block(w[j], a);
+                const int io = j >= LAG ? i : (i + MT - 1) % MT, jo = (j + NT - LAG) % NT;
+                const float s = j >= LAG ? s_now : s_before;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(d[k], s, acc[i][j][k]);
+                for (int k = 0; k < 4; ++k) acc[io][jo][k] = fmaf(d[old][k], s, acc[io][jo][k]);
+                in_order(acc[io][jo], a);
             }
         }
-        buffer_wait();
+    };
+    fetch_rows(0);
+    if (A.kblocks > 1) fetch_rows(1);
+    fetch_weights(even, 0);
+    wait_loads();
+    block_sync();
+    read_row(row, 0, 0);
+    int kb = 0;
+    for (; kb + 1 < A.kblocks; kb += 2) {
+        block(kb, even, odd);
+        block(kb + 1, odd, even);
+    }
+    if (kb < A.kblocks) block(kb, even, odd);
+#pragma unroll
+    for (int j = NT - LAG; j < NT; ++j) {
+        const int t = MT * NT - NT + j;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[MT - 1][j][k] = fmaf(d[t % SLOTS][k], s_now, acc[MT - 1][j][k]);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
