@@ -208,7 +208,7 @@ int nfe_bias_act_backward(const float* out, const float* grad, const float* grad
  *   nfe_grad_clip: g <- g * min(1, max_norm / (norm + 1e-6)), rounded once to g's type; nothing is written where the factor is 1, and
  *   a NaN norm makes every gradient NaN (torch.nn.utils.clip_grad_norm_'s behaviour).
  * data / n / dtype are HOST arrays of `count` entries: device pointer (aligned to its element), number of contiguous elements (0 is
- * allowed, at most 2^37), NFE_F32 / NFE_BF16 / NFE_F16.  Entries of one nfe_grad_clip list must not share memory (NFE_EINVAL).
+ * allowed, at most 2^34), NFE_F32 / NFE_BF16 / NFE_F16.  Entries of one nfe_grad_clip list must not share memory (NFE_EINVAL).
  * norm: one device float.  workspace: nfe_grad_workspace_bytes(count) device bytes, 8-byte aligned, no initial contents needed.
  * Same list, same bits: partial sums are joined in a fixed order.  May be captured into a graph (the list is baked in). */
 #define NFE_NORM_2 0

@@ -3,7 +3,7 @@
 //
 //   t = sqrt(sum_i sum_j g_ij^2)   (or max |g_ij|),   f = min(1, max_norm / (t + 1e-6)),   g_ij <- round(f g_ij)
 //
-// Two launches for up to GRAD_TABLE tensors: grad_reduce_kernel leaves one fp64 partial per workgroup, grad_clip_kernel adds the
+// Two launches for up to TABLE tensors: grad_reduce_kernel leaves one fp64 partial per workgroup, grad_clip_kernel adds the
 // partials in their order in every workgroup (no atomics: the same call gives the same bits) and scales.  Nothing is read or written a
 // second time when f = 1.  Both are bound by memory.  The table of tensors travels by value in the kernel's arguments, so a captured
 // call replays without a host copy.
@@ -21,26 +21,21 @@ NFE_NO_PACKED_FP32_BEGIN
 namespace nfe {
 namespace grad {
 
-constexpr int TABLE = 160;             // tensors per launch: 21 bytes each keep the kernel's arguments under 4 KB
-constexpr int CHUNK = 16384;           // elements a workgroup takes at a time (64 per thread)
+constexpr int TABLE = 256;             // tensors per launch: 14 bytes each keep the kernel's arguments under 4 KB
+constexpr int CHUNK = 4096;            // elements a workgroup takes at a time: 16 KB chunks share 2048 workgroups evenly (64 KB ones left a tail)
 constexpr int MAX_BLOCKS = 2048;       // 8 workgroups of 256 threads per CU; also the partials of one launch
 constexpr int THREADS = 256;
-constexpr long long MAX_ELEMENTS = 1ll << 37;      // of one tensor (more than the memory holds): TABLE of them stay below 2^31 chunks
+constexpr long long MAX_ELEMENTS = 1ll << 34;      // of one tensor (32 GB at least): TABLE of them stay below 2^31 chunks
 static_assert(TABLE * (MAX_ELEMENTS / CHUNK) < 0x7fffffffll, "chunk numbers are 32-bit");
 
 struct Table {
-    void* data[TABLE];
-    long long n[TABLE];
+    unsigned long long where[TABLE];   // address, type << 62
     int first[TABLE + 1];              // chunks before tensor i
-    unsigned char type[TABLE];
+    unsigned short last[TABLE];        // elements of its last chunk
     int count;
 };
-static_assert(sizeof(Table) <= 3520, "kernel arguments stay under 4 KB");
+static_assert(sizeof(Table) <= 3840, "kernel arguments stay under 4 KB");
 
-template <int TYPE> struct Elem;
-template <> struct Elem<NFE_F32> { typedef float T; };
-template <> struct Elem<NFE_BF16> { typedef __bf16 T; };
-template <> struct Elem<NFE_F16> { typedef _Float16 T; };
 template <typename T> struct alignas(16) Vec { static constexpr int N = 16 / (int)sizeof(T); T e[N]; };
 
 // |x| as bits, so that a NaN is larger than everything and survives the maximum
@@ -88,9 +83,8 @@ __device__ __forceinline__ int find_tensor(const Table& t, int chunk) {  // unif
 // A chunk as [head][16-byte vectors][tail]: views may start anywhere
 template <typename T> struct Span {
     T* p; int head, vecs, tail;
-    __device__ __forceinline__ Span(void* data, long long n, long long at) {
-        p = (T*)data + at;
-        const int len = (int)(n - at < CHUNK ? n - at : CHUNK);
+    __device__ __forceinline__ Span(void* data, int len) {
+        p = (T*)data;
         const int lead = (int)((16u - ((unsigned)(unsigned long long)p & 15u)) & 15u) / (int)sizeof(T);
         head = lead < len ? lead : len;
         vecs = (len - head) / Vec<T>::N;
@@ -98,22 +92,21 @@ template <typename T> struct Span {
     }
 };
 
-template <typename ACC, int TYPE>
-__device__ __forceinline__ void reduce_chunk(ACC& acc, void* data, long long n, long long at) {
-    typedef typename Elem<TYPE>::T T;
-    constexpr int V = Vec<T>::N;
-    const Span<T> s(data, n, at);
+template <typename T, typename ACC>
+__device__ __forceinline__ void reduce_chunk(ACC& acc, void* data, int len) {
+    constexpr int V = Vec<T>::N, U = CHUNK / (V * THREADS);
+    const Span<T> s(data, len);
     const int tid = threadIdx.x;
     if (tid < s.head) acc.add((float)s.p[tid]);
     if (tid < s.tail) acc.add((float)s.p[s.head + s.vecs * V + tid]);
     const Vec<T>* v = (const Vec<T>*)(s.p + s.head);
     int i = tid;
-    for (; i + 3 * THREADS < s.vecs; i += 4 * THREADS) {
-        Vec<T> q[4];
+    for (; i + (U - 1) * THREADS < s.vecs; i += U * THREADS) {
+        Vec<T> q[U];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) q[u] = v[i + u * THREADS];
+        for (int u = 0; u < U; ++u) q[u] = v[i + u * THREADS];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int k = 0; k < V; ++k) acc.add((float)q[u].e[k]);
         }
@@ -125,16 +118,27 @@ __device__ __forceinline__ void reduce_chunk(ACC& acc, void* data, long long n, 
     }
 }
 
-template <int TYPE>
-__device__ __forceinline__ void scale_chunk(float f, void* data, long long n, long long at) {
-    typedef typename Elem<TYPE>::T T;
-    constexpr int V = Vec<T>::N;
-    const Span<T> s(data, n, at);
+template <typename T>
+__device__ __forceinline__ void scale_chunk(float f, void* data, int len) {
+    constexpr int V = Vec<T>::N, U = CHUNK / (V * THREADS);
+    const Span<T> s(data, len);
     const int tid = threadIdx.x;
     if (tid < s.head) s.p[tid] = (T)((float)s.p[tid] * f);
     if (tid < s.tail) { T* e = s.p + s.head + s.vecs * V + tid; *e = (T)((float)*e * f); }
     Vec<T>* v = (Vec<T>*)(s.p + s.head);
-    for (int i = tid; i < s.vecs; i += THREADS) {
+    int i = tid;
+    for (; i + (U - 1) * THREADS < s.vecs; i += U * THREADS) {
+        Vec<T> q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = v[i + u * THREADS];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) q[u].e[k] = (T)((float)q[u].e[k] * f);
+            v[i + u * THREADS] = q[u];
+        }
+    }
+    for (; i < s.vecs; i += THREADS) {
         Vec<T> q = v[i];
 #pragma unroll
         for (int k = 0; k < V; ++k) q.e[k] = (T)((float)q.e[k] * f);
@@ -142,19 +146,29 @@ __device__ __forceinline__ void scale_chunk(float f, void* data, long long n, lo
     }
 }
 
+// body(type, address, elements) for every chunk of this workgroup.  Chunk numbers rise, so the tensor is looked up only when one is left.
+template <typename F>
+__device__ __forceinline__ void each_chunk(const Table& t, F body) {
+    const int chunks = t.first[t.count];
+    int i = 0, from = 0, to = 0;
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+        if (c >= to) { i = find_tensor(t, c); from = t.first[i]; to = t.first[i + 1]; }
+        const unsigned long long where = t.where[i];
+        const int type = (int)(where >> 62);
+        const long long at = (long long)(c - from) * CHUNK;
+        body(type, (char*)(where & ((1ull << 62) - 1)) + at * (type == NFE_F32 ? 4 : 2), c + 1 == to ? (int)t.last[i] : CHUNK);
+    }
+}
+
 template <typename ACC>
 __global__ __launch_bounds__(THREADS) void grad_reduce_kernel(Table t, double* __restrict__ partial) {
     __shared__ ACC lds[THREADS / 64];
     ACC acc; acc.clear();
-    const int chunks = t.first[t.count];
-    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int i = find_tensor(t, c);
-        const long long at = (long long)(c - t.first[i]) * CHUNK;
-        const int type = t.type[i];
-        if (type == NFE_F32) reduce_chunk<ACC, NFE_F32>(acc, t.data[i], t.n[i], at);
-        else if (type == NFE_BF16) reduce_chunk<ACC, NFE_BF16>(acc, t.data[i], t.n[i], at);
-        else reduce_chunk<ACC, NFE_F16>(acc, t.data[i], t.n[i], at);
-    }
+    each_chunk(t, [&](int type, void* p, int len) {
+        if (type == NFE_F32) reduce_chunk<float>(acc, p, len);
+        else if (type == NFE_BF16) reduce_chunk<__bf16>(acc, p, len);
+        else reduce_chunk<_Float16>(acc, p, len);
+    });
     acc = block_reduce(acc, lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc.partial();
 }
@@ -171,15 +185,11 @@ __global__ __launch_bounds__(THREADS) void grad_clip_kernel(Table t, const doubl
     if (!clip) return;
     const float f = (float)((double)max_norm / (total + 1e-6));
     if (f >= 1.0f) return;             // a NaN goes on and makes every gradient NaN
-    const int chunks = t.first[t.count];
-    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int i = find_tensor(t, c);
-        const long long at = (long long)(c - t.first[i]) * CHUNK;
-        const int type = t.type[i];
-        if (type == NFE_F32) scale_chunk<NFE_F32>(f, t.data[i], t.n[i], at);
-        else if (type == NFE_BF16) scale_chunk<NFE_BF16>(f, t.data[i], t.n[i], at);
-        else scale_chunk<NFE_F16>(f, t.data[i], t.n[i], at);
-    }
+    each_chunk(t, [&](int type, void* p, int len) {
+        if (type == NFE_F32) scale_chunk<float>(f, p, len);
+        else if (type == NFE_BF16) scale_chunk<__bf16>(f, p, len);
+        else scale_chunk<_Float16>(f, p, len);
+    });
 }
 
 // ---- host ------------------------------------------------------------------------------------
@@ -190,7 +200,7 @@ static int check_list(const char* who, const uint64_t* data, const int64_t* n, c
         NFE_REQUIRE(n[i] >= 0 && n[i] <= MAX_ELEMENTS, "%s: tensor %d has %lld elements", who, i, (long long)n[i]);
         NFE_REQUIRE(dtype[i] == NFE_F32 || dtype[i] == NFE_BF16 || dtype[i] == NFE_F16, "%s: tensor %d has unknown dtype %d", who, i, (int)dtype[i]);
         const int size = dtype[i] == NFE_F32 ? 4 : 2;
-        NFE_REQUIRE(n[i] == 0 || (data[i] && data[i] % size == 0), "%s: tensor %d: null or misaligned pointer", who, i);
+        NFE_REQUIRE(n[i] == 0 || (data[i] && data[i] % size == 0 && data[i] >> 62 == 0), "%s: tensor %d: null or misaligned pointer", who, i);
     }
     if (!writes) return NFE_OK;
     // two entries that share memory would be scaled by two workgroups at once
@@ -216,7 +226,9 @@ static void fill(Launch& l, const uint64_t* data, const int64_t* n, const int32_
         if (!n[at]) continue;
         const long long c = (n[at] + CHUNK - 1) / CHUNK;
         const int i = t.count++;
-        t.data[i] = (void*)data[at]; t.n[i] = n[at]; t.type[i] = (unsigned char)dtype[at]; t.first[i] = (int)chunks;
+        t.where[i] = data[at] | (unsigned long long)dtype[at] << 62;
+        t.last[i] = (unsigned short)(n[at] - (c - 1) * CHUNK);
+        t.first[i] = (int)chunks;
         chunks += c;
     }
     t.first[t.count] = (int)chunks;

@@ -5,14 +5,14 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _dev, _ptr, _stream
+from .ops import _dev, _on, _ptr, _stream
 
 MATH = {None: _lib.NFE_CONV_BF16X3, "bf16x3": _lib.NFE_CONV_BF16X3, "bf16": _lib.NFE_CONV_BF16, "fp16": _lib.NFE_CONV_F16,
         _lib.NFE_CONV_BF16X3: _lib.NFE_CONV_BF16X3, _lib.NFE_CONV_BF16: _lib.NFE_CONV_BF16, _lib.NFE_CONV_F16: _lib.NFE_CONV_F16}
 
 
 def _call(dev, rc_fn, what):
-    with torch.cuda.device(dev):
+    with _on(dev.index):
         _lib.check(rc_fn(), what)
 
 
@@ -372,6 +372,7 @@ def resize_bilinear(x, oh, ow, antialias=True):
 
 # ---- 8-bit rows and weights (include/nfe_dense.h: e4m3 values, one fp32 scale for every block of 128) -------------------------
 FP8_BLOCK = 128
+_FP8_MATMUL_ARGS = ctypes.sizeof(_lib.Fp8MatmulArgs)
 _FP8_TYPES = {torch.float32: _lib.NFE_F32, torch.bfloat16: _lib.NFE_BF16, torch.float16: _lib.NFE_F16}
 
 
@@ -379,27 +380,35 @@ def _fp8_blocks(n):
     return -(-n // FP8_BLOCK)
 
 
-def _fp8_rows(t, name, shape=(None, None)):
-    """_dev for the types the 8-bit operators read."""
+def _fp8_rows(t, name, like=None):
+    """_dev for the types the 8-bit operators read: a contiguous GPU matrix (of like's shape and type)."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _FP8_TYPES and t.dim() == 2 and (like is None or (t.shape == like.shape and t.dtype == like.dtype)):
+        return t.contiguous()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor, got {type(t)}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{name}: tensor is on {t.device}; this path runs only on the GPU (no CPU fallback)")
     if t.dtype not in _FP8_TYPES:
         raise RuntimeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
-    assert len(shape) == t.dim() and all(s is None or s == d for s, d in zip(shape, t.shape)), \
-        f"{name}: wrong shape {list(t.shape)}, expected {list(shape)}"
-    return t.contiguous()
+    expected = [None, None] if like is None else list(like.shape)
+    assert t.dim() == 2 and (like is None or t.shape == like.shape), f"{name}: wrong shape {list(t.shape)}, expected {expected}"
+    raise RuntimeError(f"{name}: expected {like.dtype}, got {t.dtype}")
 
 
-def _fp8_inference(what, *ts):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError(f"{what}: 8-bit outputs carry no gradient; detach the inputs or call it under torch.no_grad()")
+def _fp8_check(what, *ts):
+    """One device (its index is returned), and no gradient asked for."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t is not None:
+            if t.get_device() != index:
+                raise RuntimeError(f"{what}: the tensors are on several devices")
+            if t.requires_grad and torch.is_grad_enabled():
+                raise RuntimeError(f"{what}: 8-bit operands carry no gradient; detach the inputs or call it under torch.no_grad()")
+    return index
 
 
-def _same_device(what, dev, *ts):
-    if any(t is not None and t.device != dev for t in ts):
-        raise RuntimeError(f"{what}: the tensors are on several devices")
+def _address(t):
+    return t.data_ptr() if t is not None else None
 
 
 def _fp8_out(what, out, out_offset, rows, cols, dev):
@@ -408,7 +417,7 @@ def _fp8_out(what, out, out_offset, rows, cols, dev):
     if out is None:
         if out_offset:
             raise ValueError(f"{what}: out_offset needs out")
-        return torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=dev), torch.empty(blocks, rows, device=dev).t()
+        return torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=dev), torch.empty_strided((rows, blocks), (1, rows), device=dev)
     q, scale = out
     b = out_offset // FP8_BLOCK
     if out_offset % FP8_BLOCK or out_offset < 0 or q.dtype != torch.float8_e4m3fn or q.dim() != 2 or not q.is_contiguous() or q.shape[0] != rows or \
@@ -416,7 +425,8 @@ def _fp8_out(what, out, out_offset, rows, cols, dev):
             tuple(scale.shape) != (rows, q.shape[1] // FP8_BLOCK) or 0 in scale.stride():
         raise ValueError(f"{what}: out must be (q float8_e4m3fn [{rows}, W] contiguous, scale float32 [{rows}, W / {FP8_BLOCK}]) with W a multiple of "
                          f"{FP8_BLOCK} that holds {width} columns from out_offset, itself a multiple of {FP8_BLOCK}")
-    _same_device(what, dev, q, scale)
+    if q.device != dev or scale.device != dev:
+        raise RuntimeError(f"{what}: the tensors are on several devices")
     return q[:, out_offset:out_offset + width], scale[:, b:b + blocks]
 
 
@@ -425,37 +435,34 @@ def rms_norm_fp8(x, weight=None, residual=None, eps=1e-8, out=None, out_offset=0
     x [N,K] fp32 / bf16 / fp16, residual like x, weight [K] fp32.  Returns (q [N, Kp] float8_e4m3fn, scale [N, Kp / 128] fp32) - Kp is K
     rounded up to 128, the columns from K on are zero - and with a residual also h [N,K] in x's type.  y ~ q * scale per block.
     out = (q, scale) buffers and out_offset (columns, a multiple of 128) write into wider rows.  Inference only."""
-    lib = _lib.load()
     x = _fp8_rows(x, "x")
     N, K = x.shape
-    residual = _fp8_rows(residual, "residual", (N, K)) if residual is not None else None
-    if residual is not None and residual.dtype != x.dtype:
-        raise RuntimeError(f"residual: expected {x.dtype} like x, got {residual.dtype}")
+    residual = _fp8_rows(residual, "residual", x) if residual is not None else None
     weight = _dev(weight, "weight", (K,)) if weight is not None else None
-    _fp8_inference("rms_norm_fp8", x, residual, weight)
-    _same_device("rms_norm_fp8", x.device, residual, weight)
+    index = _fp8_check("rms_norm_fp8", x, residual, weight)
     if K == 0 or not eps > 0:
         raise ValueError("rms_norm_fp8: rows need at least one column and eps must be positive")
     q, scale = _fp8_out("rms_norm_fp8", out, out_offset, N, K, x.device)
     h = torch.empty_like(x) if residual is not None else None
     if N:
-        _call(x.device, lambda: lib.nfe_rms_norm_fp8(_ptr(x), _ptr(residual), _ptr(weight), _FP8_TYPES[x.dtype], N, K, float(eps), _ptr(h), _ptr(q),
-                                                     q.stride(0), _ptr(scale), scale.stride(0), scale.stride(1), _stream()), "nfe_rms_norm_fp8")
+        with _on(index):
+            _lib.check(_lib.load().nfe_rms_norm_fp8(x.data_ptr(), _address(residual), _address(weight), _FP8_TYPES[x.dtype], N, K, eps, _address(h),
+                                                    q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0), scale.stride(1), _stream()), "nfe_rms_norm_fp8")
     return (q, scale) if residual is None else (q, scale, h)
 
 
 def quantize_fp8(x, out=None, out_offset=0):
     """nfe_quantize_fp8: rms_norm_fp8 without the norm (the operand of the next layer's fp8_matmul) -> (q, scale)."""
-    lib = _lib.load()
     x = _fp8_rows(x, "x")
     N, K = x.shape
-    _fp8_inference("quantize_fp8", x)
+    index = _fp8_check("quantize_fp8", x)
     if K == 0:
         raise ValueError("quantize_fp8: rows need at least one column")
     q, scale = _fp8_out("quantize_fp8", out, out_offset, N, K, x.device)
     if N:
-        _call(x.device, lambda: lib.nfe_quantize_fp8(_ptr(x), _FP8_TYPES[x.dtype], N, K, _ptr(q), q.stride(0), _ptr(scale), scale.stride(0),
-                                                     scale.stride(1), _stream()), "nfe_quantize_fp8")
+        with _on(index):
+            _lib.check(_lib.load().nfe_quantize_fp8(x.data_ptr(), _FP8_TYPES[x.dtype], N, K, q.data_ptr(), q.stride(0), scale.data_ptr(), scale.stride(0),
+                                                    scale.stride(1), _stream()), "nfe_quantize_fp8")
     return q, scale
 
 
@@ -495,7 +502,8 @@ def fp8_weight_from(q, scale):
     q = q.contiguous()
     n, k = q.shape
     scale = _dev(scale, "scale", (_fp8_blocks(n), _fp8_blocks(k)))
-    _same_device("fp8_weight_from", q.device, scale)
+    if scale.device != q.device:
+        raise RuntimeError("fp8_weight_from: the tensors are on several devices")
     packed = _fp8_weight_buffer(lib, n, k, q.device)
     _call(q.device, lambda: lib.nfe_fp8_weight_pack(_ptr(q), n, k, _ptr(packed), _stream()), "nfe_fp8_weight_pack")
     return Fp8Weight(packed, scale.detach().clone(), n, k)
@@ -507,37 +515,34 @@ def fp8_matmul(q, scale, weight, bias=None, bias_gain=1.0, lrelu=False, out_dtyp
     out_dtype fp32 sums exact products in fp32; bf16 and fp16 use the 8-bit matrix instructions at twice the rate, whose sums over a block
     are off by less than 7 2^-13 sum|products| (typically 1.5e-5 of the result, below the output's own rounding).  q [N, Kp] float8_e4m3fn with Kp = in_features rounded up to 128 (zeros, or any finite values, from
     in_features on), scale [N, Kp / 128] fp32 of any strides (block-major, as rms_norm_fp8 returns it, is read fastest).  Inference only."""
-    lib = _lib.load()
     if not isinstance(weight, Fp8Weight):
         raise TypeError(f"fp8_matmul: weight must be an Fp8Weight (fp8_weight, fp8_weight_from), got {type(weight)}")
     if not isinstance(q, torch.Tensor) or q.dtype != torch.float8_e4m3fn:
         raise RuntimeError(f"fp8_matmul: q must be a float8_e4m3fn tensor, got {getattr(q, 'dtype', type(q))}")
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         raise RuntimeError(f"fp8_matmul: q is on {q.device}; this path runs only on the GPU (no CPU fallback)")
     if out_dtype not in _FP8_TYPES:
         raise RuntimeError(f"fp8_matmul: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
     n, k = weight.out_features, weight.in_features
     kb = _fp8_blocks(k)
-    assert q.dim() == 2 and q.shape[1] == kb * FP8_BLOCK, \
-        f"q: wrong shape {list(q.shape)}, expected [N, {kb * FP8_BLOCK}] ({k} input features in blocks of {FP8_BLOCK})"
+    width = kb * FP8_BLOCK
+    assert q.dim() == 2 and q.shape[1] == width, \
+        f"q: wrong shape {list(q.shape)}, expected [N, {width}] ({k} input features in blocks of {FP8_BLOCK})"
     N = q.shape[0]
-    if not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or tuple(scale.shape) != (N, kb):
+    if not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or scale.shape != (N, kb):
         raise RuntimeError(f"fp8_matmul: scale must be a float32 tensor [{N}, {kb}]")
     bias = _dev(bias, "bias", (n,)) if bias is not None else None
-    _fp8_inference("fp8_matmul", scale, bias)
-    _same_device("fp8_matmul", q.device, scale, weight.packed, bias)
+    index = _fp8_check("fp8_matmul", q, scale, weight.packed, bias)
     out = torch.empty(N, n, dtype=out_dtype, device=q.device)
     if N == 0:
         return out
-    if q.stride(1) != 1 or q.data_ptr() % 16 or (N > 1 and (q.stride(0) % 16 or q.stride(0) < kb * FP8_BLOCK)):
+    stride, inner = q.stride()
+    if inner != 1 or q.data_ptr() % 16 or (N > 1 and (stride % 16 or stride < width)):
         q = q.contiguous()
-    a = _lib.Fp8MatmulArgs()
-    a.struct_size = ctypes.sizeof(_lib.Fp8MatmulArgs)
-    a.m, a.n, a.k = N, n, k
-    a.q, a.q_stride = q.data_ptr(), q.stride(0) if N > 1 else kb * FP8_BLOCK
-    a.scale, a.scale_row_stride, a.scale_block_stride = scale.data_ptr(), scale.stride(0), scale.stride(1)
-    a.packed, a.w_scale = weight.packed.data_ptr(), weight.scale.data_ptr()
-    a.bias, a.bias_gain = (bias.data_ptr() if bias is not None else None), float(bias_gain)
-    a.lrelu, a.out_dtype, a.out = int(bool(lrelu)), _FP8_TYPES[out_dtype], out.data_ptr()
-    _call(q.device, lambda: lib.nfe_fp8_matmul(ctypes.byref(a), _stream()), "nfe_fp8_matmul")
+        stride = width
+    a = _lib.Fp8MatmulArgs(_FP8_MATMUL_ARGS, N, n, k, q.data_ptr(), stride if N > 1 else width, scale.data_ptr(), scale.stride(0), scale.stride(1),
+                           weight.packed.data_ptr(), weight.scale.data_ptr(), _address(bias), bias_gain, 1 if lrelu else 0, _FP8_TYPES[out_dtype],
+                           out.data_ptr())
+    with _on(index):
+        _lib.check(_lib.load().nfe_fp8_matmul(ctypes.byref(a), _stream()), "nfe_fp8_matmul")
     return out

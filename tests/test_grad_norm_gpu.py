@@ -42,7 +42,7 @@ def check_clipped(got, before, norm, max_norm):
 
 
 CASES = [
-    [1], [0, 1, 0], [3], [192], [255, 256, 257], [16383, 16384, 16385], [1 << 20], [5] * 161, [7, 0, 70001] * 110, [3_000_001, 17],
+    [1], [0, 1, 0], [3], [192], [255, 256, 257], [4095, 4096, 4097], [16383, 16384, 16385], [1 << 20], [5] * 257, [7, 0, 70001] * 110, [3_000_001, 17],
 ]
 
 
@@ -251,7 +251,7 @@ def test_refusals_without_a_gpu():
     with pytest.raises(ValueError, match="norm_type"):
         ops.grad_norm([torch.ones(3)], norm_type=1)
     lib = _lib.load()
-    assert lib.nfe_grad_workspace_bytes(0) == 0 and lib.nfe_grad_workspace_bytes(161) == 2 * lib.nfe_grad_workspace_bytes(160) > 0
+    assert lib.nfe_grad_workspace_bytes(0) == 0 and lib.nfe_grad_workspace_bytes(1000) >= lib.nfe_grad_workspace_bytes(1) > 0
     one = lambda c, v: (c * 1)(v)
     args = lambda p=64, n=4, t=0, count=1: (one(ctypes.c_uint64, p), one(ctypes.c_int64, n), one(ctypes.c_int32, t), count)
     for bad, word in ((args(n=-1), b"elements"), (args(n=1 << 40), b"elements"), (args(t=3), b"dtype"), (args(p=66), b"misaligned"), (args(p=0), b"null"),
