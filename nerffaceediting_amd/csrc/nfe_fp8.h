@@ -35,7 +35,7 @@ __device__ __forceinline__ unsigned e4m3x4(float a, float b, float c, float d) {
 // Everything between the load of x and the rounding to e4m3 (and of h to x's type) is fp32.  The maximum is taken on the bits, so a NaN or
 // an infinity in a block makes its scale NaN or infinite and every value of the block reads as NaN.
 // One row belongs to WAVES waves; a lane holds 8 neighbouring columns of every step, so 16 lanes share a scale.  STEPS > 0: the row stays
-// in registers and is read once; STEPS = 0: longer rows, read twice.  VEC: 16-byte loads (columns a multiple of 8, pointers aligned).
+// in registers and is read once; STEPS = 0: longer rows, read twice.
 // Memory-bound.
 // ------------------------------------------------------------------------------------------------
 struct NormArgs {
@@ -44,63 +44,62 @@ struct NormArgs {
     long long rows; int cols; float eps;
 };
 
-template <int TYPE, bool VEC>
-__device__ __forceinline__ void load8(float (&v)[8], const void* base, long long at, int left) {      // left: columns from here to the row's end
+// Eight neighbouring columns, `left` of them inside the row, whose start may be aligned to the element alone: the 16-byte accesses take any
+// address, so only the row's last, partial eight go one by one.
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Eight { T e[8]; };
+template <int TYPE>
+__device__ __forceinline__ void load8(float (&v)[8], const void* base, long long at, int left) {
     typedef typename Elem<TYPE>::T T;
     const T* p = (const T*)base + at;
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-    if (VEC) {
-        if (left > 0) {
-            const Vec<T, 8> r = *(const Vec<T, 8>*)p;
+    if (left >= 8) {
+        const Eight<T> r = *(const Eight<T>*)p;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = (float)r.e[k];
-        }
-    } else {
+        for (int k = 0; k < 8; ++k) v[k] = (float)r.e[k];
+    } else if (left > 0) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < 7; ++k)
             if (k < left) v[k] = (float)p[k];
     }
 }
-template <int TYPE, bool VEC>
+template <int TYPE>
 __device__ __forceinline__ void store8(const float (&v)[8], void* base, long long at, int left) {
     typedef typename Elem<TYPE>::T T;
     T* p = (T*)base + at;
-    if (VEC) {
-        if (left > 0) {
-            Vec<T, 8> r;
+    if (left >= 8) {
+        Eight<T> r;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) r.e[k] = (T)v[k];
-            *(Vec<T, 8>*)p = r;
-        }
-    } else {
+        for (int k = 0; k < 8; ++k) r.e[k] = (T)v[k];
+        *(Eight<T>*)p = r;
+    } else if (left > 0) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < 7; ++k)
             if (k < left) p[k] = (T)v[k];
     }
 }
 
-template <int TYPE, bool VEC, bool RES>
+template <int TYPE, bool RES>
 __device__ __forceinline__ void load_h(float (&v)[8], const NormArgs& a, long long row, int col) {
     const long long at = row * a.cols + col;
-    load8<TYPE, VEC>(v, a.x, at, a.cols - col);
+    load8<TYPE>(v, a.x, at, a.cols - col);
     if (RES) {
         float r[8];
-        load8<TYPE, VEC>(r, a.residual, at, a.cols - col);
+        load8<TYPE>(r, a.residual, at, a.cols - col);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] += r[k];
     }
 }
 
 // every lane of the wave takes part
-template <bool VEC, bool NORM>
+template <bool NORM>
 __device__ __forceinline__ void quantise8(float (&v)[8], const NormArgs& a, long long row, int col, float r) {
     if (NORM) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] *= r;
         if (a.weight) {
             float w[8];
-            load8<NFE_F32, VEC>(w, a.weight, col, a.cols - col);
+            load8<NFE_F32>(w, a.weight, col, a.cols - col);
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] *= w[k];
         }
@@ -123,7 +122,7 @@ __device__ __forceinline__ void quantise8(float (&v)[8], const NormArgs& a, long
     }
 }
 
-template <int TYPE, bool VEC, bool NORM, bool RES, int WAVES, int STEPS>
+template <int TYPE, bool NORM, bool RES, int WAVES, int STEPS>
 __global__ __launch_bounds__(256) void norm_fp8_kernel(NormArgs a) {
     __shared__ float part[4];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -134,17 +133,17 @@ __global__ __launch_bounds__(256) void norm_fp8_kernel(NormArgs a) {
     float v[KEEP][8], sum = 0.0f;
     if (STEPS > 0) {
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) load_h<TYPE, VEC, RES>(v[s], a, row, first + s * STRIDE);
+        for (int s = 0; s < STEPS; ++s) load_h<TYPE, RES>(v[s], a, row, first + s * STRIDE);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            if (RES) store8<TYPE, VEC>(v[s], a.h, row * a.cols + first + s * STRIDE, a.cols - (first + s * STRIDE));
+            if (RES) store8<TYPE>(v[s], a.h, row * a.cols + first + s * STRIDE, a.cols - (first + s * STRIDE));
             if (NORM)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) sum = fmaf(v[s][k], v[s][k], sum);
         }
     } else if (NORM || RES) {
         for (int col = first; col < a.cols; col += STRIDE) {
-            load_h<TYPE, VEC, RES>(v[0], a, row, col);
+            load_h<TYPE, RES>(v[0], a, row, col);
             if (NORM)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) sum = fmaf(v[0][k], v[0][k], sum);
@@ -163,39 +162,33 @@ __global__ __launch_bounds__(256) void norm_fp8_kernel(NormArgs a) {
     }
     if (STEPS > 0) {
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) quantise8<VEC, NORM>(v[s], a, row, first + s * STRIDE, r);
+        for (int s = 0; s < STEPS; ++s) quantise8<NORM>(v[s], a, row, first + s * STRIDE, r);
     } else {
         const int width = (a.cols + STRIDE - 1) / STRIDE * STRIDE;    // whole waves: quantise8 exchanges between lanes
         for (int col = first; col < width; col += STRIDE) {
-            load_h<TYPE, VEC, RES>(v[0], a, row, col);
-            if (RES) store8<TYPE, VEC>(v[0], a.h, row * a.cols + col, a.cols - col);
-            quantise8<VEC, NORM>(v[0], a, row, col, r);
+            load_h<TYPE, RES>(v[0], a, row, col);
+            if (RES) store8<TYPE>(v[0], a.h, row * a.cols + col, a.cols - col);
+            quantise8<NORM>(v[0], a, row, col, r);
         }
     }
 }
 
-template <int TYPE, bool VEC, bool NORM, bool RES>
+template <int TYPE, bool NORM, bool RES>
 static void norm_launch(const NormArgs& a, hipStream_t st) {
     const dim3 narrow((unsigned)((a.rows + 3) / 4)), wide((unsigned)a.rows), b(256);
     // a wave for a row of up to 2048 columns, four waves for a longer one
-    if (a.cols <= 512) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, VEC, NORM, RES, 1, 1>), narrow, b, 0, st, a);
-    else if (a.cols <= 1024) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, VEC, NORM, RES, 1, 2>), narrow, b, 0, st, a);
-    else if (a.cols <= 2048) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, VEC, NORM, RES, 1, 4>), narrow, b, 0, st, a);
-    else if (a.cols <= 4096) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, VEC, NORM, RES, 4, 2>), wide, b, 0, st, a);
-    else if (a.cols <= 8192) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, VEC, NORM, RES, 4, 4>), wide, b, 0, st, a);
-    else hipLaunchKernelGGL((norm_fp8_kernel<TYPE, VEC, NORM, RES, 4, 0>), wide, b, 0, st, a);
+    if (a.cols <= 512) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, NORM, RES, 1, 1>), narrow, b, 0, st, a);
+    else if (a.cols <= 1024) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, NORM, RES, 1, 2>), narrow, b, 0, st, a);
+    else if (a.cols <= 2048) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, NORM, RES, 1, 4>), narrow, b, 0, st, a);
+    else if (a.cols <= 4096) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, NORM, RES, 4, 2>), wide, b, 0, st, a);
+    else if (a.cols <= 8192) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, NORM, RES, 4, 4>), wide, b, 0, st, a);
+    else hipLaunchKernelGGL((norm_fp8_kernel<TYPE, NORM, RES, 4, 0>), wide, b, 0, st, a);
 }
 template <int TYPE>
 static void norm_dispatch(const NormArgs& a, bool norm, hipStream_t st) {
-    const uintptr_t all = (uintptr_t)a.x | (uintptr_t)a.residual | (uintptr_t)a.weight | (uintptr_t)a.h;
-    const bool vec = a.cols % 8 == 0 && all % 16 == 0;
-    if (!norm) {
-        if (vec) norm_launch<TYPE, true, false, false>(a, st); else norm_launch<TYPE, false, false, false>(a, st);
-    } else if (a.residual) {
-        if (vec) norm_launch<TYPE, true, true, true>(a, st); else norm_launch<TYPE, false, true, true>(a, st);
-    } else {
-        if (vec) norm_launch<TYPE, true, true, false>(a, st); else norm_launch<TYPE, false, true, false>(a, st);
-    }
+    if (!norm) norm_launch<TYPE, false, false>(a, st);
+    else if (a.residual) norm_launch<TYPE, true, true>(a, st);
+    else norm_launch<TYPE, true, false>(a, st);
 }
 
 // ------------------------------------------------------------------------------------------------
