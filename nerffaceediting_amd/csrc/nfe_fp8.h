@@ -21,7 +21,6 @@ template <> struct Elem<NFE_BF16> { typedef __bf16 T; };
 template <> struct Elem<NFE_F16> { typedef _Float16 T; };
 template <typename T, int N> struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Vec { T e[N]; };
 
-__device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
 __device__ __forceinline__ unsigned abs_bits(float v) { return bits_of(v) & 0x7fffffffu; }     // ordered as |v|, NaN above infinity
 // four values -> four e4m3 bytes, round to nearest even
 __device__ __forceinline__ unsigned e4m3x4(float a, float b, float c, float d) {
@@ -44,48 +43,74 @@ struct NormArgs {
     long long rows; int cols; float eps;
 };
 
-// Eight neighbouring columns, `left` of them inside the row, whose start may be aligned to the element alone: the 16-byte accesses take any
-// address, so only the row's last, partial eight go one by one.
+// A lane's eight neighbouring columns of a row.  16-byte accesses take any address, so rows of any length use them; what differs is how a wave's
+// 512 columns meet the row's end (all of it the same for every lane of the wave):
+enum Part { FULL,        // 512 columns
+            SHARED,      // fewer, and the eight columns that the last lane reads stay inside the tensor: read with the next row's first, then cleared
+            LAST,        // fewer, at the tensor's end: element by element
+            NONE };      // no column
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Eight { T e[8]; };
 template <int TYPE>
-__device__ __forceinline__ void load8(float (&v)[8], const void* base, long long at, int left) {
+__device__ __forceinline__ void load8(float (&v)[8], const void* row, int col, int cols, Part part) {
     typedef typename Elem<TYPE>::T T;
-    const T* p = (const T*)base + at;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-    if (left >= 8) {
+    const T* p = (const T*)row + col;
+    if (part == FULL) {
         const Eight<T> r = *(const Eight<T>*)p;
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = (float)r.e[k];
-    } else if (left > 0) {
+        return;
+    }
 #pragma unroll
-        for (int k = 0; k < 7; ++k)
-            if (k < left) v[k] = (float)p[k];
+    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+    if (part == NONE) return;
+    if (part == SHARED) {
+        if (col < cols) {
+            const Eight<T> r = *(const Eight<T>*)p;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = col + k < cols ? (float)r.e[k] : 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (col + k < cols) v[k] = (float)p[k];
     }
 }
 template <int TYPE>
-__device__ __forceinline__ void store8(const float (&v)[8], void* base, long long at, int left) {
+__device__ __forceinline__ void store8(const float (&v)[8], void* row, int col, int cols) {
     typedef typename Elem<TYPE>::T T;
-    T* p = (T*)base + at;
-    if (left >= 8) {
+    T* p = (T*)row + col;
+    if (col + 8 <= cols) {
         Eight<T> r;
 #pragma unroll
         for (int k = 0; k < 8; ++k) r.e[k] = (T)v[k];
         *(Eight<T>*)p = r;
-    } else if (left > 0) {
+    } else {
 #pragma unroll
         for (int k = 0; k < 7; ++k)
-            if (k < left) p[k] = (T)v[k];
+            if (col + k < cols) p[k] = (T)v[k];
     }
 }
 
+// What every lane of a wave knows of its row
+struct NormRow {
+    const NormArgs& a; long long row; const void *x, *residual; void* h; unsigned char* q; float* scale; bool shared;
+    __device__ __forceinline__ NormRow(const NormArgs& args, long long r, int size) : a(args), row(r) {
+        const long long at = r * args.cols * size;
+        x = (const char*)args.x + at; residual = (const char*)args.residual + at; h = (char*)args.h + at;
+        q = args.q + r * args.q_stride; scale = args.scale + r * args.scale_row;
+        shared = (args.rows - 1 - r) * args.cols >= 7;               // up to seven elements beyond the row belong to the tensor
+    }
+    __device__ __forceinline__ Part part(int base, bool more) const {       // of the 512 columns from `base` on
+        return base + 512 <= a.cols ? FULL : base >= a.cols ? NONE : more ? SHARED : LAST;
+    }
+};
 template <int TYPE, bool RES>
-__device__ __forceinline__ void load_h(float (&v)[8], const NormArgs& a, long long row, int col) {
-    const long long at = row * a.cols + col;
-    load8<TYPE>(v, a.x, at, a.cols - col);
+__device__ __forceinline__ void load_h(float (&v)[8], const NormRow& R, int base, int lane) {
+    const Part part = R.part(base, R.shared);
+    load8<TYPE>(v, R.x, base + lane * 8, R.a.cols, part);
     if (RES) {
         float r[8];
-        load8<TYPE>(r, a.residual, at, a.cols - col);
+        load8<TYPE>(r, R.residual, base + lane * 8, R.a.cols, part);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] += r[k];
     }
@@ -93,13 +118,15 @@ __device__ __forceinline__ void load_h(float (&v)[8], const NormArgs& a, long lo
 
 // every lane of the wave takes part
 template <bool NORM>
-__device__ __forceinline__ void quantise8(float (&v)[8], const NormArgs& a, long long row, int col, float r) {
+__device__ __forceinline__ void quantise8(float (&v)[8], const NormRow& R, int base, int lane, float r) {
+    if (base >= R.a.cols) return;
+    const int col = base + lane * 8;
     if (NORM) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] *= r;
-        if (a.weight) {
+        if (R.a.weight) {
             float w[8];
-            load8<NFE_F32>(w, a.weight, col, a.cols - col);
+            load8<NFE_F32>(w, R.a.weight, col, R.a.cols, R.part(base, false));
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] *= w[k];
         }
@@ -107,52 +134,48 @@ __device__ __forceinline__ void quantise8(float (&v)[8], const NormArgs& a, long
     unsigned m = bits_of(SMALLEST);
 #pragma unroll
     for (int k = 0; k < 8; ++k) m = umax(m, abs_bits(v[k]));
-#pragma unroll
-    for (int off = 1; off < 16; off <<= 1) m = umax(m, wave_xor(m, off));
+    m = row_max(m);
     const float scale = float_of(m) / E4M3_MAX;
     const float inv = 1.0f / scale;
-    if (col < a.q_stride) {
+    if (col < (R.a.cols + BLOCK - 1) / BLOCK * BLOCK) {
         uint2 w;
         w.x = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
         w.y = e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-        if (col < (a.cols + BLOCK - 1) / BLOCK * BLOCK) {
-            *(uint2*)(a.q + row * a.q_stride + col) = w;
-            if (((col >> 3) & 15) == 0) a.scale[row * a.scale_row + (long long)(col / BLOCK) * a.scale_block] = scale;
-        }
+        *(uint2*)(R.q + col) = w;
+        if ((lane & 15) == 0) R.scale[(long long)(col / BLOCK) * R.a.scale_block] = scale;
     }
 }
 
 template <int TYPE, bool NORM, bool RES, int WAVES, int STEPS>
 __global__ __launch_bounds__(256) void norm_fp8_kernel(NormArgs a) {
     __shared__ float part[4];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const long long row = WAVES == 1 ? (long long)blockIdx.x * 4 + wave : (long long)blockIdx.x;
     if (row >= a.rows) return;                                        // WAVES == 1 only: no barrier below then
-    const int first = (WAVES == 1 ? 0 : wave * 512) + lane * 8;
+    const NormRow R(a, row, (int)sizeof(typename Elem<TYPE>::T));
+    const int first = WAVES == 1 ? 0 : wave * 512;
     constexpr int STRIDE = WAVES * 512, KEEP = STEPS > 0 ? STEPS : 1;
     float v[KEEP][8], sum = 0.0f;
     if (STEPS > 0) {
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) load_h<TYPE, RES>(v[s], a, row, first + s * STRIDE);
+        for (int s = 0; s < STEPS; ++s) load_h<TYPE, RES>(v[s], R, first + s * STRIDE, lane);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            if (RES) store8<TYPE>(v[s], a.h, row * a.cols + first + s * STRIDE, a.cols - (first + s * STRIDE));
+            if (RES) store8<TYPE>(v[s], R.h, first + s * STRIDE + lane * 8, a.cols);
             if (NORM)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) sum = fmaf(v[s][k], v[s][k], sum);
         }
-    } else if (NORM || RES) {
-        for (int col = first; col < a.cols; col += STRIDE) {
-            load_h<TYPE, RES>(v[0], a, row, col);
-            if (NORM)
+    } else if (NORM) {
+        for (int base = first; base < a.cols; base += STRIDE) {
+            load_h<TYPE, RES>(v[0], R, base, lane);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) sum = fmaf(v[0][k], v[0][k], sum);
+            for (int k = 0; k < 8; ++k) sum = fmaf(v[0][k], v[0][k], sum);
         }
     }
     float r = 1.0f;
     if (NORM) {
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) sum += wave_xor(sum, off);
+        sum = wave_sum(sum);
         if (WAVES > 1) {
             if (lane == 0) part[wave] = sum;
             block_sync();
@@ -162,13 +185,12 @@ __global__ __launch_bounds__(256) void norm_fp8_kernel(NormArgs a) {
     }
     if (STEPS > 0) {
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) quantise8<NORM>(v[s], a, row, first + s * STRIDE, r);
+        for (int s = 0; s < STEPS; ++s) quantise8<NORM>(v[s], R, first + s * STRIDE, lane, r);
     } else {
-        const int width = (a.cols + STRIDE - 1) / STRIDE * STRIDE;    // whole waves: quantise8 exchanges between lanes
-        for (int col = first; col < width; col += STRIDE) {
-            load_h<TYPE, RES>(v[0], a, row, col);
-            if (RES) store8<TYPE>(v[0], a.h, row * a.cols + col, a.cols - col);
-            quantise8<NORM>(v[0], a, row, col, r);
+        for (int base = first; base < a.cols; base += STRIDE) {
+            load_h<TYPE, RES>(v[0], R, base, lane);
+            if (RES) store8<TYPE>(v[0], R.h, base + lane * 8, a.cols);
+            quantise8<NORM>(v[0], R, base, lane, r);
         }
     }
 }
@@ -179,6 +201,7 @@ static void norm_launch(const NormArgs& a, hipStream_t st) {
     // a wave for a row of up to 2048 columns, four waves for a longer one
     if (a.cols <= 512) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, NORM, RES, 1, 1>), narrow, b, 0, st, a);
     else if (a.cols <= 1024) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, NORM, RES, 1, 2>), narrow, b, 0, st, a);
+    else if (a.cols <= 1536) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, NORM, RES, 1, 3>), narrow, b, 0, st, a);
     else if (a.cols <= 2048) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, NORM, RES, 1, 4>), narrow, b, 0, st, a);
     else if (a.cols <= 4096) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, NORM, RES, 4, 2>), wide, b, 0, st, a);
     else if (a.cols <= 8192) hipLaunchKernelGGL((norm_fp8_kernel<TYPE, NORM, RES, 4, 4>), wide, b, 0, st, a);
