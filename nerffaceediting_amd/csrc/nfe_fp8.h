@@ -1,6 +1,8 @@
 // 8-bit dense operators (e4m3 values, one fp32 scale for every block of 128): RMS norm / quantisation of rows, packing of weights and the
 // product of the two.  Part of nfe_dense.hip's code object, beside the fp32 fully-connected layers they are the 8-bit form of.
 #pragma once
+#include <algorithm>
+
 #include "nfe_dense.h"
 #include "nfe_wave.h"
 
@@ -19,7 +21,25 @@ template <int TYPE> struct Elem;
 template <> struct Elem<NFE_F32> { typedef float T; };
 template <> struct Elem<NFE_BF16> { typedef __bf16 T; };
 template <> struct Elem<NFE_F16> { typedef _Float16 T; };
-template <typename T, int N> struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Vec { T e[N]; };
+// N neighbouring values at any address that T allows, in 8- and 16-byte accesses.  (A struct of N elements is loaded and stored element by
+// element as soon as the compiler has taken it apart.)
+template <typename T, int N> struct Vec { T e[N]; };
+typedef unsigned any8 __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned any16 __attribute__((ext_vector_type(4), aligned(2)));
+struct Two16 { any16 v[2]; };
+template <typename T, int N> __device__ __forceinline__ Vec<T, N> load_any(const T* p) {
+    constexpr int BYTES = N * (int)sizeof(T);
+    static_assert(BYTES == 16 || BYTES == 32, "size");
+    if constexpr (BYTES == 16) return __builtin_bit_cast(Vec<T, N>, *(const any16*)p);
+    else { const Two16 t = {{*(const any16*)p, *((const any16*)p + 1)}}; return __builtin_bit_cast(Vec<T, N>, t); }
+}
+template <typename T, int N> __device__ __forceinline__ void store_any(T* p, const Vec<T, N>& r) {
+    constexpr int BYTES = N * (int)sizeof(T);
+    static_assert(BYTES == 8 || BYTES == 16 || BYTES == 32, "size");
+    if constexpr (BYTES == 8) *(any8*)p = __builtin_bit_cast(any8, r);
+    else if constexpr (BYTES == 16) *(any16*)p = __builtin_bit_cast(any16, r);
+    else { const Two16 t = __builtin_bit_cast(Two16, r); *(any16*)p = t.v[0]; *((any16*)p + 1) = t.v[1]; }
+}
 
 __device__ __forceinline__ unsigned abs_bits(float v) { return bits_of(v) & 0x7fffffffu; }     // ordered as |v|, NaN above infinity
 // four values -> four e4m3 bytes, round to nearest even
@@ -49,13 +69,12 @@ enum Part { FULL,        // 512 columns
             SHARED,      // fewer, and the eight columns that the last lane reads stay inside the tensor: read with the next row's first, then cleared
             LAST,        // fewer, at the tensor's end: element by element
             NONE };      // no column
-template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Eight { T e[8]; };
 template <int TYPE>
 __device__ __forceinline__ void load8(float (&v)[8], const void* row, int col, int cols, Part part) {
     typedef typename Elem<TYPE>::T T;
     const T* p = (const T*)row + col;
     if (part == FULL) {
-        const Eight<T> r = *(const Eight<T>*)p;
+        const Vec<T, 8> r = load_any<T, 8>(p);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = (float)r.e[k];
         return;
@@ -65,7 +84,7 @@ __device__ __forceinline__ void load8(float (&v)[8], const void* row, int col, i
     if (part == NONE) return;
     if (part == SHARED) {
         if (col < cols) {
-            const Eight<T> r = *(const Eight<T>*)p;
+            const Vec<T, 8> r = load_any<T, 8>(p);
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = col + k < cols ? (float)r.e[k] : 0.0f;
         }
@@ -80,10 +99,10 @@ __device__ __forceinline__ void store8(const float (&v)[8], void* row, int col, 
     typedef typename Elem<TYPE>::T T;
     T* p = (T*)row + col;
     if (col + 8 <= cols) {
-        Eight<T> r;
+        Vec<T, 8> r;
 #pragma unroll
         for (int k = 0; k < 8; ++k) r.e[k] = (T)v[k];
-        *(Eight<T>*)p = r;
+        store_any<T, 8>(p, r);
     } else {
 #pragma unroll
         for (int k = 0; k < 7; ++k)
@@ -275,7 +294,7 @@ __global__ __launch_bounds__(256) void weight_fp8_kernel(const void* w, const un
 struct MatmulArgs {
     const unsigned char* a; const float* a_scale; const unsigned char* w; const float* w_scale; const float* bias; void* out;
     long long a_stride, scale_row, scale_block;
-    int m, n, kblocks, lrelu, out_type, vec_out; float bias_gain;
+    int m, n, kblocks, lrelu, out_type; float bias_gain;
 };
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -314,87 +333,140 @@ __device__ __forceinline__ f32x4 mfma_block(const Frag<true>& w, const Frag<true
 
 // No instruction: what follows and needs `a` comes after what made `acc`.  Without it the compiler issues a block's products first and its
 // additions after them, and spills.
+__device__ __forceinline__ void in_order(f32x4& acc, i32x4& a) { asm volatile("" : "+v"(acc), "+v"(a)); }
 __device__ __forceinline__ void in_order(f32x4& acc, Frag<false>& a) { asm volatile("" : "+v"(acc), "+v"(a.v)); }
 __device__ __forceinline__ void in_order(f32x4& acc, Frag<true>& a) { asm volatile("" : "+v"(acc), "+v"(a.v[0]), "+v"(a.v[1]), "+v"(a.v[2]), "+v"(a.v[3])); }
 
 template <int TYPE>
-__device__ __forceinline__ void store4(const float (&v)[4], void* out, long long at, int left, int vec) {
+__device__ __forceinline__ void store4(const float (&v)[4], void* out, long long at, int left) {
     typedef typename Elem<TYPE>::T T;
     T* p = (T*)out + at;
-    if (vec) {                                    // the row length is a multiple of 4: all four columns are inside
-        Vec<T, 4> r;
+    Vec<T, 4> r;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r.e[i] = (T)v[i];
-        *(Vec<T, 4>*)p = r;
+    for (int i = 0; i < 4; ++i) r.e[i] = (T)v[i];
+    if (left >= 4) {                              // one store at any alignment: rows of any length
+        store_any<T, 4>(p, r);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < left) p[i] = (T)v[i];
+        for (int i = 0; i < 3; ++i)
+            if (i < left) p[i] = r.e[i];
     }
 }
-// columns n .. n + 3 of row m
-__device__ __forceinline__ void finish4(const MatmulArgs& A, f32x4 s, int m, int n) {
-    if (m >= A.m) return;
-    if (n >= A.n) return;
-    float v[4];
+// What a lane needs to finish columns n .. n + 3 of any row
+struct Finish {
+    int n, left; float bias[4];
+    __device__ __forceinline__ Finish(const MatmulArgs& A, int column) : n(column), left(A.n - column) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[i] = s[i];
-        if (A.bias) v[i] = fmaf(A.bias[n + i < A.n ? n + i : A.n - 1], A.bias_gain, v[i]);
+        for (int i = 0; i < 4; ++i) bias[i] = 0.0f;
+        if (A.bias)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bias[i] = A.bias[n + i < A.n ? n + i : A.n - 1] * A.bias_gain;
     }
-    if (A.lrelu)
+    template <int TYPE> __device__ __forceinline__ void store(const MatmulArgs& A, const f32x4& s, int m) const {
+        if (m >= A.m) return;
+        if (left <= 0) return;
+        float v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (v[i] < 0.0f ? v[i] * 0.2f : v[i]) * 1.4142135623730951f;      // bias_act 'lrelu': alpha 0.2, gain sqrt(2)
-    const long long at = (long long)m * A.n + n;
-    if (A.out_type == NFE_F32) store4<NFE_F32>(v, A.out, at, A.n - n, A.vec_out);
-    else if (A.out_type == NFE_BF16) store4<NFE_BF16>(v, A.out, at, A.n - n, A.vec_out);
-    else store4<NFE_F16>(v, A.out, at, A.n - n, A.vec_out);
+        for (int i = 0; i < 4; ++i) v[i] = s[i] + bias[i];
+        if (A.lrelu)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = (v[i] < 0.0f ? v[i] * 0.2f : v[i]) * 1.4142135623730951f;      // bias_act 'lrelu': alpha 0.2, gain sqrt(2)
+        store4<TYPE>(v, A.out, (long long)m * A.n + n, left);
+    }
+};
+// each(store) calls store(sums, row) for whatever it has: one copy of it for each output type
+template <bool WIDE, typename F> __device__ __forceinline__ void finish(const MatmulArgs& A, const Finish& f, F each) {
+    if (WIDE) each([&](const f32x4& s, int m) { f.store<NFE_F32>(A, s, m); });
+    else if (A.out_type == NFE_BF16) each([&](const f32x4& s, int m) { f.store<NFE_BF16>(A, s, m); });
+    else each([&](const f32x4& s, int m) { f.store<NFE_F16>(A, s, m); });
 }
 
-// Few rows.  A workgroup of WAVES waves owns 16 columns of the output and 16 MT rows; the waves share the K blocks, read both operands
-// straight into registers and join their sums through LDS.  Every weight is read once: bound by that.
-template <bool WIDE, int MT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void matmul_rows_kernel(MatmulArgs A) {
-    __shared__ f32x4 part[WAVES][MT][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int nt = blockIdx.x, m0 = blockIdx.y * (16 * MT);
-    const int g = lane >> 4, r = lane & 15;
-    const unsigned char* wp = A.w + (long long)nt * A.kblocks * 2048 + lane * 16;
+// Few rows, or few tiles.  A workgroup of WAVES waves owns 16 MT rows x 16 NT columns; its waves share the K blocks, read both operands straight
+// into registers, one block ahead, and join their sums through LDS in the order of the waves.  Bound by reading: every weight once for each 16 MT
+// rows, every row once for each 16 NT columns.
+template <bool WIDE, int MT, int NT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, MT * NT >= 8 ? 2 : MT * NT >= 4 ? 3 : 4) void matmul_rows_kernel(MatmulArgs A) {
+    __shared__ f32x4 part[WAVES][MT * NT][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    const int nt0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT), last = (A.n + 15) / 16 - 1;
     const unsigned char* ap[MT]; const float* sp[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int m = m0 + 16 * t + r;
+    for (int i = 0; i < MT; ++i) {
+        const int m = m0 + 16 * i + r;
         const long long row = m < A.m ? m : A.m - 1;
-        ap[t] = A.a + row * A.a_stride + g * 16;
-        sp[t] = A.a_scale + row * A.scale_row;
+        ap[i] = A.a + row * A.a_stride + g * 16;
+        sp[i] = A.a_scale + row * A.scale_row;
     }
-    const float* ws = A.w_scale + (long long)(nt >> 3) * A.kblocks;
-    f32x4 acc[MT];
+    const unsigned char* wp[NT]; const float* wsp[NT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int kb = wave; kb < A.kblocks; kb += WAVES) {
-        Frag<WIDE> w;
-        w.set(*(const i32x4*)(wp + (long long)kb * 2048), *(const i32x4*)(wp + (long long)kb * 2048 + 1024));
-        const float sw = ws[kb];
+    for (int j = 0; j < NT; ++j) {
+        const int nt = nt0 + j < last ? nt0 + j : last;
+        wp[j] = A.w + (long long)nt * A.kblocks * 2048;
+        wsp[j] = A.w_scale + (long long)(nt >> 3) * A.kblocks;
+    }
+    struct Block { i32x4 a[MT][2], w[NT][2]; float sa[MT], sw[NT]; };
+    auto fetch = [&](Block& b, int kb) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            Frag<WIDE> a;
-            a.set(*(const i32x4*)(ap[t] + (long long)kb * 128), *(const i32x4*)(ap[t] + (long long)kb * 128 + 64));
-            const float s = sp[t][kb * A.scale_block] * sw;
-            const f32x4 d = mfma_block(w, a);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(d[i], s, acc[t][i]);
+        for (int j = 0; j < NT; ++j) {
+            b.w[j][0] = *(const i32x4*)(wp[j] + (long long)kb * 2048 + lane * 16);
+            b.w[j][1] = *(const i32x4*)(wp[j] + (long long)kb * 2048 + 1024 + lane * 16);
+            b.sw[j] = wsp[j][kb];
         }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            b.a[i][0] = *(const i32x4*)(ap[i] + (long long)kb * 128);
+            b.a[i][1] = *(const i32x4*)(ap[i] + (long long)kb * 128 + 64);
+            b.sa[i] = sp[i][kb * A.scale_block];
+        }
+    };
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto multiply = [&](const Block& b) {
+        Frag<WIDE> w[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) w[j].set(b.w[j][0], b.w[j][1]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            i32x4 lo = b.a[i][0];
+            if (i > 0)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) in_order(acc[i - 1][j], lo);
+            Frag<WIDE> a;
+            a.set(lo, b.a[i][1]);
+            f32x4 d[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) d[j] = mfma_block(w[j], a);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const float s = b.sa[i] * b.sw[j];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(d[j][k], s, acc[i][j][k]);
+            }
+        }
+    };
+    Block even, odd;
+    int kb = wave;
+    if (kb < A.kblocks) fetch(even, kb);
+    for (; kb + WAVES < A.kblocks; kb += 2 * WAVES) {
+        fetch(odd, kb + WAVES);
+        multiply(even);
+        if (kb + 2 * WAVES < A.kblocks) fetch(even, kb + 2 * WAVES);
+        multiply(odd);
     }
+    if (kb < A.kblocks) multiply(even);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
     block_sync();
-    for (int e = threadIdx.x; e < MT * 64; e += 64 * WAVES) {
-        const int t = e >> 6, l = e & 63;
-        f32x4 s = part[0][t][l];
+    for (int t = wave; t < MT * NT; t += WAVES) {
+        f32x4 s = part[0][t][lane];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) s += part[w][t][l];
-        finish4(A, s, m0 + 16 * t + (l & 15), nt * 16 + (l >> 4) * 4);
+        for (int w = 1; w < WAVES; ++w) s += part[w][t][lane];
+        finish<WIDE>(A, Finish(A, (nt0 + t % NT) * 16 + g * 4), [&](auto store) { store(s, m0 + 16 * (t / NT) + r); });
     }
 }
 
@@ -527,7 +599,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs
                 const int io = j >= LAG ? i : (i + MT - 1) % MT, jo = (j + NT - LAG) % NT;
                 const float s = j >= LAG ? s_now : s_before;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) acc[io][jo][k] = fmaf(d[old][k], s, acc[io][jo][k]);
+                for (int e = 0; e < 4; ++e) acc[io][jo][e] = fmaf(d[old][e], s, acc[io][jo][e]);
                 in_order(acc[io][jo], a);
             }
         }
@@ -539,7 +611,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs
     block_sync();
     read_row(row, 0, 0);
     int kb = 0;
-    for (; kb + 1 < A.kblocks; kb += 2) {
+    for (; kb + 1 < A.kblocks; kb += 2) {                // in pairs, so that no weights are moved between registers
         block(kb, even, odd);
         block(kb + 1, odd, even);
     }
@@ -548,12 +620,31 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs
     for (int j = NT - LAG; j < NT; ++j) {
         const int t = MT * NT - NT + j;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) acc[MT - 1][j][k] = fmaf(d[t % SLOTS][k], s_now, acc[MT - 1][j][k]);
+        for (int e = 0; e < 4; ++e) acc[MT - 1][j][e] = fmaf(d[t % SLOTS][e], s_now, acc[MT - 1][j][e]);
     }
+    // A wave's results go through its part of the ring, 16-byte chunk c of row r at c ^ r, and come back as whole row segments: full cache
+    // lines to store, and one copy of the finishing code (straight from the accumulators it was most of the kernel's code, and a call's first
+    // workgroups wait for every line of it).
+    constexpr int CHUNKS = 4 * NT, TILE = MT * NT * 1024 * WM * WN, RING = 4 * BM * 128, PARTS = TILE > RING ? TILE / RING : 1, PM = MT / PARTS;
+    static_assert(MT % PARTS == 0 && TILE <= RING * PARTS, "epilogue");
+    unsigned char* mine = &rows[0][0] + wave * (PM * NT * 1024);
+    const int c = lane & (CHUNKS - 1), first = lane / CHUNKS;
+    const Finish f(A, n0 + c * 4);
+    block_sync();
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int p = 0; p < PARTS; ++p) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) finish4(A, acc[i][j], m0 + (wm * MT + i) * 16 + r, n0 + 16 * j + 4 * g);
+        for (int i = 0; i < PM; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) *(f32x4*)(mine + ((i * 16 + r) * CHUNKS + ((j * 4 + g) ^ (r & (CHUNKS - 1)))) * 16) = acc[p * PM + i][j];
+        finish<WIDE>(A, f, [&](auto store) {
+#pragma unroll 4
+            for (int t = 0; t < PM * NT; ++t) {
+                const int row = t * (64 / CHUNKS) + first;
+                store(*(const f32x4*)(mine + (row * CHUNKS + (c ^ (row & (CHUNKS - 1)))) * 16), m0 + (wm * MT + p * PM) * 16 + row);
+            }
+        });
+    }
 }
 
 template <bool WIDE, int WM, int WN, int MT, int NT>
@@ -565,20 +656,42 @@ static int tile_launch(const MatmulArgs& A, hipStream_t st) {
     return NFE_OK;
 }
 
-// Offsets inside a tile are 32-bit: 256 rows of up to 2^23 bytes (and scales that far apart); anything wider stays on the rows kernel.
+template <bool WIDE, int MT, int NT, int WAVES>
+static int rows_launch(const MatmulArgs& A, hipStream_t st) {
+    const long long x = ((long long)A.n + 16 * NT - 1) / (16 * NT), y = ((long long)A.m + 16 * MT - 1) / (16 * MT);
+    NFE_REQUIRE(y <= 65535, "nfe_fp8_matmul: m=%d is too large for rows %lld bytes apart", A.m, A.a_stride);
+    hipLaunchKernelGGL((matmul_rows_kernel<WIDE, MT, NT, WAVES>), dim3((unsigned)x, (unsigned)y), dim3(64 * WAVES), 0, st, A);
+    return NFE_OK;
+}
+// Which kernel.  Rows kernels: the largest tile that still gives every CU a workgroup (their waves share K, so a short chain of blocks stays
+// short).  Among the widest of them and the tile kernels: the least of rounds x (time of one workgroup's K block), rounds = workgroups /
+// CUs rounded up, but not less than what a lone workgroup takes for a block (loads' latency).  us measured on 256 CUs, K block = 128:
+//                       a workgroup's block, CU full   alone     measured
+//   32 x 64   rows   8-bit 0.23, widened 0.28       0.29, 0.33   128 x 8192 x 8192: 29.5 (bf16), 31.3 us (fp32); 64 rows: 18.6, 20.9
+//   64 x 64   tile         0.30          0.36       0.62, 0.67   512 x 4096 x 4096: 21.7, 27.6
+//   128 x 128 tile         0.66          1.15       0.82, 1.20   2048^3: 15.0, 22.8
+//   256 x 256 tile         2.00                     2.00         4096^3: 67
+//   128 x 256 tile                       1.94             1.94   4096^3: 124
+// E.g. 10000 x 512 x 1024 fp32: 64 x 64 5 rounds x 0.36, 128 x 128 2 x 1.15, 128 x 256 1 x 1.94: 18.5, 24.5, 21.8 us measured.
+// Offsets inside a tile are 32-bit: 256 rows of up to 2^23 bytes (and scales that far apart); anything wider stays on the rows kernels.
 template <bool WIDE>
 static int matmul_launch(const MatmulArgs& A, hipStream_t st) {
-    const unsigned nt = (unsigned)((A.n + 15) / 16);
-    const long long mt = ((long long)A.m + 63) / 64;
+    const int cus = num_cus();
+    auto count = [&](int bm, int bn) { return (((long long)A.m + bm - 1) / bm) * (((long long)A.n + bn - 1) / bn); };
     const bool near = A.a_stride <= (1 << 23) && A.scale_row <= (1 << 21);
-    if (A.m <= 16) hipLaunchKernelGGL((matmul_rows_kernel<WIDE, 1, 8>), dim3(nt), dim3(512), 0, st, A);
-    else if (A.m <= 32) hipLaunchKernelGGL((matmul_rows_kernel<WIDE, 2, 8>), dim3(nt), dim3(512), 0, st, A);
-    else if (A.m <= 64 || !near) {
-        NFE_REQUIRE(mt <= 65535, "nfe_fp8_matmul: m=%d is too large for rows %lld bytes apart", A.m, A.a_stride);
-        hipLaunchKernelGGL((matmul_rows_kernel<WIDE, 4, 8>), dim3(nt, (unsigned)mt), dim3(512), 0, st, A);
-    } else if (!WIDE && ((long long)A.m + 255) / 256 * (((long long)A.n + 255) / 256) >= 200) return tile_launch<false, 2, 4, 8, 4>(A, st);
-    else return tile_launch<WIDE, 2, 2, 4, 4>(A, st);
-    return NFE_OK;
+    if (count(32, 64) < cus || !near) {
+        if (count(32, 32) < cus && near) return count(16, 32) < cus ? rows_launch<WIDE, 1, 1, 8>(A, st) : rows_launch<WIDE, 1, 2, 8>(A, st);
+        if (near) return rows_launch<WIDE, 2, 2, 8>(A, st);
+        return rows_launch<WIDE, 2, 4, 4>(A, st);
+    }
+    auto cost = [&](int bm, int bn, double full, double alone) { return std::max(alone, full * (double)((count(bm, bn) + cus - 1) / cus)); };
+    const double rows = WIDE ? cost(32, 64, 0.28, 0.33) : cost(32, 64, 0.23, 0.29), small = WIDE ? cost(64, 64, 0.36, 0.67) : cost(64, 64, 0.30, 0.62),
+                 middle = WIDE ? cost(128, 128, 1.15, 1.20) : cost(128, 128, 0.66, 0.82), large = WIDE ? cost(128, 256, 1.94, 1.94) : cost(256, 256, 2.0, 2.0);
+    const double best = std::min(std::min(rows, small), std::min(middle, large));
+    if (rows == best) return rows_launch<WIDE, 2, 4, 4>(A, st);
+    if (small == best) return tile_launch<WIDE, 2, 2, 2, 2>(A, st);
+    if (middle == best) return tile_launch<WIDE, 2, 4, 4, 2>(A, st);
+    return WIDE ? tile_launch<true, 2, 4, 4, 4>(A, st) : tile_launch<false, 2, 4, 8, 4>(A, st);
 }
 
 static int check_rows(const char* who, long long rows, int cols) {
@@ -658,7 +771,7 @@ extern "C" int nfe_fp8_matmul(const nfe_fp8_matmul_args* p, nfe_stream_t stream)
     const int size = p->out_dtype == NFE_F32 ? 4 : 2;
     NFE_REQUIRE((uintptr_t)p->out % size == 0, "nfe_fp8_matmul: misaligned out");
     MatmulArgs A{(const unsigned char*)p->q, p->scale, (const unsigned char*)p->packed, p->w_scale, p->bias, p->out, p->q_stride, p->scale_row_stride,
-                 p->scale_block_stride, p->m, p->n, kblocks, p->lrelu, p->out_dtype, p->n % 4 == 0 && (uintptr_t)p->out % (4 * size) == 0, p->bias_gain};
+                 p->scale_block_stride, p->m, p->n, kblocks, p->lrelu, p->out_dtype, p->bias_gain};
     if (int rc = p->out_dtype == NFE_F32 ? matmul_launch<true>(A, (hipStream_t)stream) : matmul_launch<false>(A, (hipStream_t)stream)) return rc;
     NFE_CHECK_LAUNCH("nfe_fp8_matmul");
     return NFE_OK;
