@@ -25,6 +25,7 @@ constexpr int TABLE = 256;             // tensors per launch: 14 bytes each keep
 constexpr int CHUNK = 4096;            // elements a workgroup takes at a time: 16 KB chunks share 2048 workgroups evenly (64 KB ones left a tail)
 constexpr int MAX_BLOCKS = 2048;       // 8 workgroups of 256 threads per CU; also the partials of one launch
 constexpr int THREADS = 256;
+constexpr int SMALL = 4;               // chunks that one workgroup takes alone
 constexpr long long MAX_ELEMENTS = 1ll << 34;      // of one tensor (32 GB at least): TABLE of them stay below 2^31 chunks
 static_assert(TABLE * (MAX_ELEMENTS / CHUNK) < 0x7fffffffll, "chunk numbers are 32-bit");
 
@@ -161,16 +162,41 @@ __device__ __forceinline__ void each_chunk(const Table& t, F body) {
 }
 
 template <typename ACC>
-__global__ __launch_bounds__(THREADS) void grad_reduce_kernel(Table t, double* __restrict__ partial) {
-    __shared__ ACC lds[THREADS / 64];
+__device__ __forceinline__ ACC reduce_all(const Table& t, ACC* lds) {
     ACC acc; acc.clear();
     each_chunk(t, [&](int type, void* p, int len) {
         if (type == NFE_F32) reduce_chunk<float>(acc, p, len);
         else if (type == NFE_BF16) reduce_chunk<__bf16>(acc, p, len);
         else reduce_chunk<_Float16>(acc, p, len);
     });
-    acc = block_reduce(acc, lds);
+    return block_reduce(acc, lds);
+}
+__device__ __forceinline__ void scale_all(const Table& t, float f) {
+    each_chunk(t, [&](int type, void* p, int len) {
+        if (type == NFE_F32) scale_chunk<float>(f, p, len);
+        else if (type == NFE_BF16) scale_chunk<__bf16>(f, p, len);
+        else scale_chunk<_Float16>(f, p, len);
+    });
+}
+__device__ __forceinline__ float factor(double max_norm, double total) { return (float)(max_norm / (total + 1e-6)); }
+
+template <typename ACC>
+__global__ __launch_bounds__(THREADS) void grad_reduce_kernel(Table t, double* __restrict__ partial) {
+    __shared__ ACC lds[THREADS / 64];
+    const ACC acc = reduce_all(t, lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc.partial();
+}
+
+// A handful of chunks: one workgroup does all of it in one launch (2 x 96 values: 13.4 -> 10.4 us a call, of which 3.6 us are a launch)
+template <typename ACC>
+__global__ __launch_bounds__(THREADS) void grad_small_kernel(Table t, int clip, float max_norm, float* __restrict__ norm) {
+    __shared__ ACC lds[THREADS / 64];
+    const double total = reduce_all<ACC>(t, lds).norm();
+    if (threadIdx.x == 0) *norm = (float)total;
+    if (!clip) return;
+    const float f = factor(max_norm, total);
+    if (f >= 1.0f) return;             // every value has been read: block_reduce has a barrier
+    scale_all(t, f);
 }
 
 // clip = 0: the norm alone (one workgroup, an empty table)
@@ -183,13 +209,9 @@ __global__ __launch_bounds__(THREADS) void grad_clip_kernel(Table t, const doubl
     const double total = block_reduce(acc, lds).norm();
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
     if (!clip) return;
-    const float f = (float)((double)max_norm / (total + 1e-6));
+    const float f = factor(max_norm, total);
     if (f >= 1.0f) return;             // a NaN goes on and makes every gradient NaN
-    each_chunk(t, [&](int type, void* p, int len) {
-        if (type == NFE_F32) scale_chunk<float>(f, p, len);
-        else if (type == NFE_BF16) scale_chunk<__bf16>(f, p, len);
-        else scale_chunk<_Float16>(f, p, len);
-    });
+    scale_all(t, f);
 }
 
 // ---- host ------------------------------------------------------------------------------------
@@ -240,6 +262,13 @@ static int run(const char* who, const uint64_t* data, const int64_t* n, const in
                hipStream_t st) {
     int n_partial = 0;
     Launch l;
+    int end = 0;
+    fill(l, data, n, dtype, count, end);
+    if (end == count && l.blocks <= SMALL) {
+        hipLaunchKernelGGL((grad_small_kernel<ACC>), dim3(1), dim3(THREADS), 0, st, l.t, clip, max_norm, norm);
+        NFE_CHECK_LAUNCH(who);
+        return NFE_OK;
+    }
     for (int at = 0; at < count;) {
         fill(l, data, n, dtype, count, at);
         if (!l.blocks) break;

@@ -1,6 +1,7 @@
 """Tensor-level wrappers over the C ABI: validate, allocate outputs with torch, pass raw pointers and
 the current HIP stream.  PyTorch is plumbing here (memory + stream); all arithmetic is in the library."""
 import ctypes
+from array import array
 
 import torch
 
@@ -558,16 +559,16 @@ def _grad_call(what, tensors, norm_type, max_norm=None):
     try:             # one pass per property: a list of 180 tensors costs less than the kernels that read it
         types = [_GRAD_TYPES[t.dtype] for t in ts]
         index = ts[0].get_device()
-        plain = index >= 0 and all([t.is_contiguous() for t in ts]) and all([t.get_device() == index for t in ts]) and not any([t.requires_grad for t in ts])
+        plain = index >= 0 and False not in [t.is_contiguous() and t.get_device() == index and not t.requires_grad for t in ts]
     except (AttributeError, KeyError, RuntimeError):
         plain = False
     if not plain:
         ts = _grad_refuse(what, ts, max_norm is not None)
         types = [_GRAD_TYPES[t.dtype] for t in ts]
         index = ts[0].get_device()
-    data = (ctypes.c_uint64 * n)(*[t.data_ptr() for t in ts])
-    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in ts])
-    types = (ctypes.c_int32 * n)(*types)
+    data = (ctypes.c_uint64 * n).from_buffer(array("Q", [t.data_ptr() for t in ts]))
+    sizes = (ctypes.c_int64 * n).from_buffer(array("q", [t.numel() for t in ts]))
+    types = (ctypes.c_int32 * n).from_buffer(array("i", types))
     with _on(index):
         dev = ts[0].device
         norm = torch.empty((), device=dev)
