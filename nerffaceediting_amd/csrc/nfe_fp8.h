@@ -477,8 +477,8 @@ __global__ __launch_bounds__(64 * WAVES, MT * NT >= 8 ? 2 : MT * NT >= 4 ? 3 : 4
 //   * the weights' fragments, already in operand order, go straight from L2 to registers: through LDS they would take it beyond its bandwidth;
 //   * a wave multiplies its MT x NT fragments, MT + NT reads for MT NT matrix instructions; a product is scaled into its accumulator
 //     LAG instructions after it was issued, so that the vector unit works under the matrix unit.
-// Block kb begins with a wait for every load issued a whole block before (rows of kb + 1, weights of kb) and issues the rows of kb + 2 and the
-// weights of kb + 1.  The one barrier, in the middle of the block, says that the rows of kb + 1 are there for everybody, so no wave stops
+// Block kb begins with a wait for every load issued in the block before (rows of kb + 1, weights of kb) and issues the rows of kb + 2 and, a
+// quarter into it, the weights of kb + 1.  The one barrier, in the middle of the block, says that the rows of kb + 1 are there for everybody, so no wave stops
 // between blocks; and as nobody is left in block kb - 2 then, buffer (kb + 2) % 4 is free when block kb begins.
 // Workgroups b, b + 8, .. run on one XCD: each XCD gets a contiguous range of tiles, GROUP row tiles deep, so that its L2 serves both operands.
 // LDS-DMA: 64 lanes x 16 (4) bytes from base + offset into 1 KiB (256 bytes) at dst.  Inline assembly, because the compiler would wait for the DMA
@@ -582,10 +582,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs
 #pragma unroll
         for (int j = 0; j < NT; ++j) w[j].set(raw.v[j][0], raw.v[j][1]);
         const float sw = raw.scale;
-        if (kb + 1 < A.kblocks) fetch_weights(next, kb + 1);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             if (i == MT / 2) block_sync();
+            if (i == MT / 4) { if (kb + 1 < A.kblocks) fetch_weights(next, kb + 1); }      // not in one burst with the rows: 8192^3 484 -> 468 us
             Frag<WIDE> a;
             a.set(row.lo, row.hi);
             s_before = s_now;
@@ -651,7 +651,7 @@ template <bool WIDE, int WM, int WN, int MT, int NT>
 static int tile_launch(const MatmulArgs& A, hipStream_t st) {
     constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN;
     const long long tm = ((long long)A.m + BM - 1) / BM, tn = ((long long)A.n + BN - 1) / BN;
-    NFE_REQUIRE(tm * tn <= 0x7fffffffll, "nfe_fp8_matmul: m=%d n=%d are too large", A.m, A.n);
+    NFE_REQUIRE(tm * tn * (64 * WM * WN) <= 0xffffffffll, "nfe_fp8_matmul: m=%d n=%d are too large", A.m, A.n);      // work items of a launch
     hipLaunchKernelGGL((matmul_tile_kernel<WIDE, WM, WN, MT, NT>), dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), 0, st, A, (int)tm, (int)tn);
     return NFE_OK;
 }
@@ -707,14 +707,24 @@ static int norm_entry(const char* who, NormArgs& a, int dtype, bool norm, nfe_st
     const int width = (a.cols + BLOCK - 1) / BLOCK * BLOCK;
     NFE_REQUIRE(a.q_stride >= width && a.q_stride % 8 == 0 && (uintptr_t)a.q % 8 == 0, "%s: q rows must be 8-byte aligned and at least %d bytes apart", who, width);
     NFE_REQUIRE(!norm || a.eps > 0.0f, "%s: eps must be positive", who);
-    if (dtype == NFE_F32) norm_dispatch<NFE_F32>(a, norm, (hipStream_t)stream);
-    else if (dtype == NFE_BF16) norm_dispatch<NFE_BF16>(a, norm, (hipStream_t)stream);
-    else norm_dispatch<NFE_F16>(a, norm, (hipStream_t)stream);
-    NFE_CHECK_LAUNCH(who);
+    const long long rows = a.rows, most = 1 << 22;                    // 2^32 work items are a launch's limit
+    for (long long at = 0; at < rows; at += most) {
+        NormArgs part = a;
+        const long long first = at * a.cols * (dtype == NFE_F32 ? 4 : 2);
+        part.rows = rows - at < most ? rows - at : most;
+        part.x = (const char*)a.x + first;
+        if (a.residual) { part.residual = (const char*)a.residual + first; part.h = (char*)a.h + first; }
+        part.q = a.q + at * a.q_stride;
+        part.scale = a.scale + at * a.scale_row;
+        if (dtype == NFE_F32) norm_dispatch<NFE_F32>(part, norm, (hipStream_t)stream);
+        else if (dtype == NFE_BF16) norm_dispatch<NFE_BF16>(part, norm, (hipStream_t)stream);
+        else norm_dispatch<NFE_F16>(part, norm, (hipStream_t)stream);
+        NFE_CHECK_LAUNCH(who);
+    }
     return NFE_OK;
 }
 static int check_weight(const char* who, int n, int k) {
-    NFE_REQUIRE(n > 0 && k > 0 && n <= (1 << 23) && k <= (1 << 30), "%s: bad sizes n=%d k=%d", who, n, k);
+    NFE_REQUIRE(n > 0 && k > 0 && n <= 65535 * BLOCK && k <= (1 << 30), "%s: bad sizes n=%d k=%d", who, n, k);
     return NFE_OK;
 }
 

@@ -481,7 +481,7 @@ def _fp8_weight_buffer(lib, n, k, dev):
 
 def fp8_weight(weight, gain=1.0):
     """nfe_fp8_weight_quantize: weight [out, in] (fp32 / bf16 / fp16), rounded to e4m3 with one scale for every 128 x 128 block; gain
-    multiplies the scales (FullyConnectedLayer's weight_gain)."""
+    multiplies the scales (FullyConnectedLayer's weight_gain).  A NaN or an infinity makes its whole block NaN."""
     lib = _lib.load()
     weight = _fp8_rows(weight, "weight").detach()
     n, k = weight.shape

@@ -578,7 +578,10 @@ def _grad_call(what, tensors, norm_type, max_norm=None):
             _lib.check(lib.nfe_grad_norm(data, sizes, types, n, _NORM_TYPES[norm_type], *tail), "nfe_grad_norm")
         else:
             _lib.check(lib.nfe_grad_clip(data, sizes, types, n, _NORM_TYPES[norm_type], float(max_norm), *tail), "nfe_grad_clip")
-            torch.autograd.graph.increment_version(ts)
+            try:
+                torch.autograd.graph.increment_version(ts)
+            except RuntimeError:                              # tensors made under inference_mode have no version
+                torch.autograd.graph.increment_version([t for t in ts if not t.is_inference()])
     return norm
 
 

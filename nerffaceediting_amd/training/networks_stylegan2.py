@@ -56,12 +56,14 @@ class FullyConnectedLayer(torch.nn.Module):
 
     def forward_fp8(self, q, scale):
         """forward() on 8-bit rows (dense_ops.rms_norm_fp8 / quantize_fp8) and this layer's weights rounded to e4m3 -> fp32."""
-        key = (self.weight.data_ptr(), self.weight._version, tuple(self.weight.shape))
-        if getattr(self, "_fp8_key", None) != key:
-            self._fp8 = dense_ops.fp8_weight(self.weight.detach(), gain=self.weight_gain)
-            _publish()
-            self._fp8_key = key
-        return dense_ops.fp8_matmul(q, scale, self._fp8, None if self.bias is None else self.bias.detach(), self.bias_gain, self.activation == "lrelu")
+        src, version, packed = getattr(self, "_fp8", (None, None, None))
+        w = self.weight
+        if src is None or src.data_ptr() != w.data_ptr() or version != w._version or src.device != w.device or src.shape != w.shape:
+            packed = dense_ops.fp8_weight(w.detach(), gain=self.weight_gain)
+            if not torch.cuda.is_current_stream_capturing():      # in a graph the image is made by every replay, and is there only then
+                _publish()
+                self._fp8 = (w.detach(), w._version, packed)      # keeps the parameter's memory: its address cannot come back with other values
+        return dense_ops.fp8_matmul(q, scale, packed, None if self.bias is None else self.bias.detach(), self.bias_gain, self.activation == "lrelu")
 
     def extra_repr(self):
         return f"in_features={self.in_features:d}, out_features={self.out_features:d}, activation={self.activation:s}"

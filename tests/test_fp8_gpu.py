@@ -444,3 +444,52 @@ def test_refusals_without_a_gpu():
     for kw, word in ((dict(rows=0), b"rows"), (dict(cols=0), b"cols"), (dict(dtype=9), b"dtype"), (dict(res=64), b"pairs"), (dict(stride=200), b"at least"),
                      (dict(stride=260), b"aligned"), (dict(q=4097), b"aligned"), (dict(q=None), b"null"), (dict(eps=0.0), b"eps")):
         assert norm(**kw) == -1 and word in err(), (kw, err())
+
+
+@pytest.mark.gpu
+def test_mapping_network_fp8_weight_image(dev):
+    """The packed image follows the parameter: in-place change, replaced storage, and a first call inside a graph capture."""
+    from nerffaceediting_amd.training.networks_stylegan2 import FullyConnectedLayer
+    from nerffaceediting_amd import dense_ops
+    torch.manual_seed(3)
+    layer = FullyConnectedLayer(256, 130).to(dev)
+    q, s = dense_ops.quantize_fp8(torch.randn(9, 256, device=dev))
+    want = lambda: dense_ops.fp8_matmul(q, s, dense_ops.fp8_weight(layer.weight.detach(), gain=layer.weight_gain), layer.bias.detach(), layer.bias_gain)
+    side = torch.cuda.Stream(device=dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = layer.forward_fp8(q, s)
+    assert torch.equal(layer.forward_fp8(q, s), want())                # the capture ran nothing
+    for i in range(3):
+        with torch.no_grad():
+            layer.weight.mul_(1.5)
+        g.replay()
+        ref = want()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref) and torch.equal(layer.forward_fp8(q, s), ref)
+    for _ in range(2):
+        layer.weight.data = torch.randn(130, 256, device=dev)
+    assert torch.equal(layer.forward_fp8(q, s), want())
+    layer.weight = torch.nn.Parameter(torch.randn(130, 256, device=dev))
+    assert torch.equal(layer.forward_fp8(q, s), want())
+
+
+@pytest.mark.gpu
+def test_many_rows_and_wide_strides(dev):
+    """More rows than one launch of the norm takes (2^22), and row strides beyond what a tile's 32-bit offsets reach (2^23 bytes)."""
+    from nerffaceediting_amd import dense_ops
+    rows = (1 << 22) + 37
+    x = torch.randn(rows, 9, device=dev, dtype=torch.bfloat16)
+    q, s = dense_ops.quantize_fp8(x)
+    at = torch.tensor([0, 1, (1 << 22) - 1, 1 << 22, (1 << 22) + 1, rows - 1], device=dev)
+    check_rows(q[at], s[at], x[at].double().cpu(), 9, rel=2.0 ** -22)
+    m, n, k, stride = 130, 70, 300, (1 << 23) + 16
+    qs, ss, wq, ws = make_mm(m, n, k, seed=5)
+    store = torch.zeros(m * stride, dtype=torch.uint8, device=dev)
+    wide = store.as_strided((m, 384), (stride, 1))
+    wide.copy_(qs.view(torch.uint8))
+    W = dense_ops.fp8_weight_from(wq.to(dev), ws.to(dev))
+    got = dense_ops.fp8_matmul(wide.view(torch.float8_e4m3fn), ss.to(dev), W)
+    want, mag = mm64(qs, ss, wq, ws, dev)
+    check_mm(got, want, mag, k)
