@@ -666,7 +666,9 @@ static int rows_launch(const MatmulArgs& A, hipStream_t st) {
     hipLaunchKernelGGL((matmul_rows_kernel<WIDE, MT, NT, WAVES>), dim3((unsigned)x, (unsigned)y), dim3(64 * WAVES), 0, st, A);
     return NFE_OK;
 }
-// Which kernel.  Rows kernels: the largest tile that still gives every CU a workgroup (their waves share K, so a short chain of blocks stays
+// Which kernel.  Up to 16 rows: one tile of rows, as a second would hold none, and eight waves to share K (against 32 x 64 on four waves, fp32
+// outputs: 16 x 16384 x 4096 15.9 -> 12.7 us, 16 x 20000 x 8192 32.7 -> 27.1, 1 x 65536 x 2048 22.4 -> 21.1; bf16 13.9 -> 12.6, 31.1 -> 26.8, 21.9 -> 21.1).
+// More: rows kernels: the largest tile that still gives every CU a workgroup (their waves share K, so a short chain of blocks stays
 // short).  Among the widest of them and the tile kernels: the least of rounds x (time of one workgroup's K block), rounds = workgroups /
 // CUs rounded up, but not less than what a lone workgroup takes for a block (loads' latency).  us measured on 256 CUs, K block = 128:
 //                       a workgroup's block, CU full   alone     measured
@@ -682,6 +684,7 @@ static int matmul_launch(const MatmulArgs& A, hipStream_t st) {
     const int cus = num_cus();
     auto count = [&](int bm, int bn) { return (((long long)A.m + bm - 1) / bm) * (((long long)A.n + bn - 1) / bn); };
     const bool near = A.a_stride <= (1 << 23) && A.scale_row <= (1 << 21);
+    if (A.m <= 16) return count(16, 32) < cus ? rows_launch<WIDE, 1, 1, 8>(A, st) : rows_launch<WIDE, 1, 2, 8>(A, st);
     if (count(32, 64) < cus || !near) {
         if (count(32, 32) < cus && near) return count(16, 32) < cus ? rows_launch<WIDE, 1, 1, 8>(A, st) : rows_launch<WIDE, 1, 2, 8>(A, st);
         if (near) return rows_launch<WIDE, 2, 2, 8>(A, st);

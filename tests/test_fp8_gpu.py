@@ -187,7 +187,7 @@ def check_mm(got, want, mag, k, extra=None):
 
 MM = [(1, 512, 1024), (1, 1, 1), (2, 3, 5), (16, 16, 128), (15, 17, 127), (17, 33, 129), (31, 500, 640), (33, 64, 256), (64, 512, 512), (65, 129, 1000),
       (100, 1000, 300), (128, 128, 128), (129, 257, 1031), (255, 256, 2048), (256, 255, 1920), (500, 513, 512), (1000, 100, 4096), (5, 4100, 8192),
-      (1, 130, 20000), (300, 48, 16384), (1500, 1031, 384)]
+      (1, 130, 20000), (300, 48, 16384), (1500, 1031, 384), (3, 8230, 300), (16, 16500, 1100), (20, 16500, 400)]
 
 
 @pytest.mark.gpu
