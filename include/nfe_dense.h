@@ -209,7 +209,8 @@ int nfe_bias_act_backward(const float* out, const float* grad, const float* grad
  *   a NaN norm makes every gradient NaN (torch.nn.utils.clip_grad_norm_'s behaviour).
  * data / n / dtype are HOST arrays of `count` entries: device pointer (aligned to its element), number of contiguous elements (0 is
  * allowed, at most 2^34), NFE_F32 / NFE_BF16 / NFE_F16.  Entries of one nfe_grad_clip list must not share memory (NFE_EINVAL).
- * norm: one device float.  workspace: nfe_grad_workspace_bytes(count) device bytes, 8-byte aligned, no initial contents needed.
+ * norm: one device float.  workspace: nfe_grad_workspace_bytes(count) device bytes, 8-byte aligned, no initial contents needed, overwritten
+ * from its first byte: a buffer of the call's own, not one that holds a render call's status or that another call may use at the same time.
  * Same list, same bits: partial sums are joined in a fixed order.  May be captured into a graph (the list is baked in). */
 #define NFE_NORM_2 0
 #define NFE_NORM_MAX 1

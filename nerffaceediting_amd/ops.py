@@ -572,7 +572,9 @@ def _grad_call(what, tensors, norm_type, max_norm=None):
     with _on(index):
         dev = ts[0].device
         norm = torch.empty((), device=dev)
-        ws = _workspace(dev, lib.nfe_grad_workspace_bytes(n))
+        # partial sums of this call alone: _workspace begins with the render calls' status words, and a call from another host thread may
+        # put its launches between this one's
+        ws = torch.empty(lib.nfe_grad_workspace_bytes(n), dtype=torch.uint8, device=dev)
         tail = (norm.data_ptr(), ws.data_ptr(), ws.numel(), _stream())
         if max_norm is None:
             _lib.check(lib.nfe_grad_norm(data, sizes, types, n, _NORM_TYPES[norm_type], *tail), "nfe_grad_norm")

@@ -262,3 +262,65 @@ def test_refusals_without_a_gpu():
     assert lib.nfe_grad_clip(*args(), 0, -1.0, 256, 256, 1 << 30, None) == -1 and b"max_norm" in lib.nfe_last_error()
     two = ((ctypes.c_uint64 * 2)(64, 72), (ctypes.c_int64 * 2)(4, 4), (ctypes.c_int32 * 2)(0, 0), 2)
     assert lib.nfe_grad_clip(*two, 0, 1.0, 256, 256, 1 << 30, None) == -1 and b"share memory" in lib.nfe_last_error()
+
+
+@pytest.mark.gpu
+def test_clipping_leaves_the_render_calls_status_alone(dev):
+    """optimize_planes clips between the backward and the callback: what ops.render and ops.render_backward left for
+    render_call_status() and render_handoff_aborts() stays, a clean status and a lost hand-off alike."""
+    from nerffaceediting_amd import ops
+    from tests.test_render_backward_gpu import _editing_size_case
+    args, kw = _editing_size_case(dev)                                   # one forward
+    grads = [g for g in ops.render_backward(*args, need=(True, True), **kw)]
+    small, many = torch.ones(5, device=dev), [torch.ones(9000, device=dev) for _ in range(300)]
+
+    def clip_all():
+        for norm_type in (2, float("inf")):
+            ops.grad_norm(grads, norm_type)
+            ops.clip_grad_norm([small] + grads, 1.0, norm_type)
+            ops.clip_grad_norm(many, 1e-3, norm_type)
+
+    def lost():
+        return [ops.render_handoff_aborts(backward=b) for b in (False, True)]
+
+    clip_all()
+    assert lost() == [0, 0]
+    ops.render_call_status()
+    ops.render_call_status(backward=True)
+    words = ops._workspaces[(0, ops._stream())].view(torch.int32)
+    planted = words[:64].clone()
+    words[0], words[2], words[6] = 5, 3, 4                               # the counts of a forward's two passes and of a backward
+    before = lost()
+    assert all(before)
+    clip_all()
+    assert lost() == before
+    with pytest.raises(RuntimeError, match="hand-offs"):
+        ops.render_call_status()
+    words[:64].copy_(planted)
+    assert lost() == [0, 0]
+
+
+@pytest.mark.gpu
+def test_two_threads_on_one_stream(dev):
+    """Calls from two host threads interleave their launches on the stream that they share: each scales by its own norm."""
+    import threading
+    from nerffaceediting_amd import ops
+    n, rounds, bad = 40000, 300, []
+
+    def work(value):
+        t = torch.full((n,), value, device=dev)
+        norm, got = value * math.sqrt(n), []
+        for _ in range(rounds):
+            g = t.clone()
+            got.append((ops.clip_grad_norm([g], 0.5 * norm), g[0], g[-1]))
+        for total, a, b in got:
+            for x, want in ((total, norm), (a, 0.5 * value), (b, 0.5 * value)):
+                if abs(float(x) - want) > 2.0 ** -20 * want:
+                    bad.append((value, float(x), want))
+
+    threads = [threading.Thread(target=work, args=(v,)) for v in (1.0, 64.0)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad[:3]
