@@ -56,11 +56,15 @@ class FullyConnectedLayer(torch.nn.Module):
 
     def forward_fp8(self, q, scale):
         """forward() on 8-bit rows (dense_ops.rms_norm_fp8 / quantize_fp8) and this layer's weights rounded to e4m3 -> fp32."""
-        src, version, packed = getattr(self, "_fp8", (None, None, None))
         w = self.weight
-        if src is None or src.data_ptr() != w.data_ptr() or version != w._version or src.device != w.device or src.shape != w.shape:
+        if torch.cuda.is_current_stream_capturing():
+            # A graph makes its own image, in its own memory, at every replay: so it follows the parameter as the fp32 layer does, and no
+            # later eager call can free what it reads.
             packed = dense_ops.fp8_weight(w.detach(), gain=self.weight_gain)
-            if not torch.cuda.is_current_stream_capturing():      # in a graph the image is made by every replay, and is there only then
+        else:
+            src, version, packed = getattr(self, "_fp8", (None, None, None))
+            if src is None or src.data_ptr() != w.data_ptr() or version != w._version or src.device != w.device or src.shape != w.shape:
+                packed = dense_ops.fp8_weight(w.detach(), gain=self.weight_gain)
                 _publish()
                 self._fp8 = (w.detach(), w._version, packed)      # keeps the parameter's memory: its address cannot come back with other values
         return dense_ops.fp8_matmul(q, scale, packed, None if self.bias is None else self.bias.detach(), self.bias_gain, self.activation == "lrelu")
