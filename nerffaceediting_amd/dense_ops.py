@@ -471,6 +471,17 @@ class Fp8Weight:
 
     def __init__(self, packed, scale, out_features, in_features):
         self.packed, self.scale, self.out_features, self.in_features = packed, scale, int(out_features), int(in_features)
+        self._stream = self._current_stream()
+
+    def _current_stream(self):
+        return torch._C._cuda_getCurrentRawStream(self.packed.get_device()) if self.packed.is_cuda else None
+
+    def used(self):
+        """For a holder that may drop the weights while a product on the current stream has still to read them: on a stream other than the one
+        they were made on, their memory is handed out again only after what that stream has been given so far."""
+        if self._stream != self._current_stream():
+            for t in (self.packed, self.scale):
+                t.record_stream(torch.cuda.current_stream(t.device))
 
 
 def _fp8_weight_buffer(lib, n, k, dev):

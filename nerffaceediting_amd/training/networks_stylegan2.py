@@ -67,6 +67,7 @@ class FullyConnectedLayer(torch.nn.Module):
                 packed = dense_ops.fp8_weight(w.detach(), gain=self.weight_gain)
                 _publish()
                 self._fp8 = (w.detach(), w._version, packed)      # keeps the parameter's memory: its address cannot come back with other values
+            packed.used()
         return dense_ops.fp8_matmul(q, scale, packed, None if self.bias is None else self.bias.detach(), self.bias_gain, self.activation == "lrelu")
 
     def extra_repr(self):

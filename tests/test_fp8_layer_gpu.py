@@ -66,3 +66,28 @@ def test_replays_outlive_the_eager_image(dev):
             torch.cuda.synchronize()
             assert torch.equal(out, ref), i
         del junk
+
+
+@pytest.mark.gpu
+def test_image_replaced_while_another_stream_reads_it(dev):
+    """Image made on one stream, product waiting on another, image replaced there: what the first stream allocates next is not the image that
+    the product has still to read."""
+    layer, q, s, want = make(dev)
+    layer.forward_fp8(q, s)
+    ref = want()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream(device=dev)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)                                    # about 0.1 s
+        out = layer.forward_fp8(q, s)
+        done = torch.cuda.Event()
+        done.record()
+        new = (layer.weight.detach() * 2).clone()
+        layer.weight = torch.nn.Parameter(new)
+        size = layer._fp8[2].packed.numel()
+        del layer._fp8                                                    # what replacing it does, without the wait of making the next one
+    junk = [torch.full((size,), 0x7F, dtype=torch.uint8, device=dev) for _ in range(8)]      # e4m3 NaN
+    torch.cuda.current_stream(dev).synchronize()
+    assert not done.query()                                               # the product has not run yet
+    torch.cuda.synchronize()
+    assert torch.equal(out, ref) and len(junk) == 8
