@@ -31,11 +31,12 @@ def _pack_cached(module, weight, conv_math=None):
     return getattr(module, attr)
 
 
-def _publish():
+def _publish(device=None):
     """A cached device buffer is about to become visible to every later call, possibly on another HIP stream (apps.StreamRing):
-    finish the kernels that fill it first.  Happens once per parameter version; skipped while a hipGraph is being captured."""
+    finish the kernels that fill it first.  Happens once per parameter version; skipped while a hipGraph is being captured.
+    device: where the kernels run, if that need not be the current one."""
     if not torch.cuda.is_current_stream_capturing():
-        torch.cuda.current_stream().synchronize()
+        torch.cuda.current_stream(device).synchronize()
 
 
 class FullyConnectedLayer(torch.nn.Module):
@@ -57,7 +58,7 @@ class FullyConnectedLayer(torch.nn.Module):
     def forward_fp8(self, q, scale):
         """forward() on 8-bit rows (dense_ops.rms_norm_fp8 / quantize_fp8) and this layer's weights rounded to e4m3 -> fp32."""
         w = self.weight
-        if torch.cuda.is_current_stream_capturing():
+        if w.is_cuda and torch.cuda.is_current_stream_capturing():
             # A graph makes its own image, in its own memory, at every replay: so it follows the parameter as the fp32 layer does, and no
             # later eager call can free what it reads.
             packed = dense_ops.fp8_weight(w.detach(), gain=self.weight_gain)
@@ -65,7 +66,7 @@ class FullyConnectedLayer(torch.nn.Module):
             src, version, packed = getattr(self, "_fp8", (None, None, None))
             if src is None or src.data_ptr() != w.data_ptr() or version != w._version or src.device != w.device or src.shape != w.shape:
                 packed = dense_ops.fp8_weight(w.detach(), gain=self.weight_gain)
-                _publish()
+                _publish(w.device)
                 self._fp8 = (w.detach(), w._version, packed)      # keeps the parameter's memory: its address cannot come back with other values
             packed.used()
         return dense_ops.fp8_matmul(q, scale, packed, None if self.bias is None else self.bias.detach(), self.bias_gain, self.activation == "lrelu")

@@ -91,3 +91,30 @@ def test_image_replaced_while_another_stream_reads_it(dev):
     assert not done.query()                                               # the product has not run yet
     torch.cuda.synchronize()
     assert torch.equal(out, ref) and len(junk) == 8
+
+
+def test_image_is_finished_on_its_own_device(monkeypatch):
+    """Before the image is kept, the stream that makes it is waited for: the one of the weights' device, whichever device is current."""
+    from nerffaceediting_amd.training import networks_stylegan2 as net
+    layer = net.FullyConnectedLayer(8, 4)
+    waited = []
+
+    class Stream:
+        def __init__(self, device):
+            self.device = device
+
+        def synchronize(self):
+            waited.append(self.device)
+
+    class Image:
+        def used(self):
+            pass
+
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        layer.forward_fp8(None, None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream(device))
+    monkeypatch.setattr(net.dense_ops, "fp8_weight", lambda w, gain: Image())
+    monkeypatch.setattr(net.dense_ops, "fp8_matmul", lambda *a: None)
+    layer.forward_fp8(None, None)
+    assert waited == [layer.weight.device]
