@@ -71,6 +71,10 @@ class FullyConnectedLayer(torch.nn.Module):
             packed.used()
         return dense_ops.fp8_matmul(q, scale, packed, None if self.bias is None else self.bias.detach(), self.bias_gain, self.activation == "lrelu")
 
+    def __getstate__(self):
+        """Copies and pickles make their own weight image: a loaded parameter's version starts anew, so it says nothing about this one's."""
+        return {k: v for k, v in self.__dict__.items() if k != "_fp8"}
+
     def extra_repr(self):
         return f"in_features={self.in_features:d}, out_features={self.out_features:d}, activation={self.activation:s}"
 

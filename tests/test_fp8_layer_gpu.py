@@ -118,3 +118,43 @@ def test_image_is_finished_on_its_own_device(monkeypatch):
     monkeypatch.setattr(net.dense_ops, "fp8_matmul", lambda *a: None)
     layer.forward_fp8(None, None)
     assert waited == [layer.weight.device]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["save", "deepcopy"])
+def test_copies_of_a_layer_make_their_own_image(dev, how):
+    """Weights changed after the image was made, then the module saved and loaded (or copied): a loaded parameter's version starts anew, and
+    must not meet the version that the image was made at."""
+    import copy
+    from nerffaceediting_amd import dense_ops
+    for bumps in range(3):
+        layer, q, s, _ = make(dev)
+        with torch.no_grad():
+            for _ in range(bumps):
+                layer.weight.add_(0.25)
+            layer.forward_fp8(q, s)
+            layer.weight.mul_(-3.0)
+        if how == "save":
+            file = io.BytesIO()
+            torch.save(layer, file)
+            file.seek(0)
+            other = torch.load(file, weights_only=False)
+        else:
+            other = copy.deepcopy(layer)
+        ref = dense_ops.fp8_matmul(q, s, dense_ops.fp8_weight(other.weight.detach(), gain=other.weight_gain), other.bias.detach(), other.bias_gain)
+        assert torch.equal(other.forward_fp8(q, s), ref), bumps
+        assert torch.equal(layer.forward_fp8(q, s), ref), bumps
+
+
+def test_a_saved_layer_carries_no_image():
+    import copy
+    from nerffaceediting_amd.training.networks_stylegan2 import FullyConnectedLayer
+    layer = FullyConnectedLayer(8, 4)
+    plain = set(layer.__dict__)
+    layer._fp8 = (layer.weight.detach(), layer.weight._version, "image")
+    file = io.BytesIO()
+    torch.save(layer, file)
+    file.seek(0)
+    for other in (torch.load(file, weights_only=False), copy.deepcopy(layer)):
+        assert set(other.__dict__) == plain and torch.equal(other.weight, layer.weight)
+    assert layer._fp8[2] == "image"
