@@ -63,11 +63,12 @@ class FullyConnectedLayer(torch.nn.Module):
             # later eager call can free what it reads.
             packed = dense_ops.fp8_weight(w.detach(), gain=self.weight_gain)
         else:
-            src, version, packed = getattr(self, "_fp8", (None, None, None))
-            if src is None or src.data_ptr() != w.data_ptr() or version != w._version or src.device != w.device or src.shape != w.shape:
+            src, made_for, packed = getattr(self, "_fp8", (None, None, None))
+            key = (w.data_ptr(), w._version, w.device, w.dtype, w.shape, w.stride(), self.weight_gain)
+            if src is None or src[0] is not w or made_for != key:  # another parameter's versions say nothing about this one's
                 packed = dense_ops.fp8_weight(w.detach(), gain=self.weight_gain)
                 _publish(w.device)
-                self._fp8 = (w.detach(), w._version, packed)      # keeps the parameter's memory: its address cannot come back with other values
+                self._fp8 = ((w, w.detach()), key, packed)        # keeps the parameter's memory: its address cannot come back with other values
             packed.used()
         return dense_ops.fp8_matmul(q, scale, packed, None if self.bias is None else self.bias.detach(), self.bias_gain, self.activation == "lrelu")
 

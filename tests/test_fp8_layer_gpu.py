@@ -158,3 +158,28 @@ def test_a_saved_layer_carries_no_image():
     for other in (torch.load(file, weights_only=False), copy.deepcopy(layer)):
         assert set(other.__dict__) == plain and torch.equal(other.weight, layer.weight)
     assert layer._fp8[2] == "image"
+
+
+@pytest.mark.gpu
+def test_image_follows_strides_and_gain(dev):
+    """Changes that leave the parameter's address, shape and version as they were."""
+    layer, q, s, want = make(dev, n=256)
+    layer.forward_fp8(q, s)
+    layer.weight.data = layer.weight.data.t()
+    assert torch.equal(layer.forward_fp8(q, s), want())
+    layer.weight_gain = layer.weight_gain * 3
+    assert torch.equal(layer.forward_fp8(q, s), want())
+
+
+@pytest.mark.gpu
+def test_image_follows_a_new_parameter_on_the_same_memory(dev):
+    """Parameter(layer.weight.data) starts its versions at 0 again; setting the kept image to None makes it anew."""
+    layer, q, s, want = make(dev)
+    layer.forward_fp8(q, s)
+    with torch.no_grad():
+        layer.weight.mul_(-2.0)
+    layer.weight = torch.nn.Parameter(layer.weight.data, requires_grad=False)
+    assert torch.equal(layer.forward_fp8(q, s), want())
+    layer.weight.data.mul_(0.5)
+    layer._fp8 = (None, None, None)
+    assert torch.equal(layer.forward_fp8(q, s), want())
