@@ -58,9 +58,9 @@ class FullyConnectedLayer(torch.nn.Module):
     def forward_fp8(self, q, scale):
         """forward() on 8-bit rows (dense_ops.rms_norm_fp8 / quantize_fp8) and this layer's weights rounded to e4m3 -> fp32."""
         w = self.weight
-        if w.is_cuda and torch.cuda.is_current_stream_capturing():
-            # A graph makes its own image, in its own memory, at every replay: so it follows the parameter as the fp32 layer does, and no
-            # later eager call can free what it reads.
+        if w.is_inference() or w.is_cuda and torch.cuda.is_current_stream_capturing():
+            # Inference tensors have no version to know an image by.  A graph makes its own image, in its own memory, at every replay: so it
+            # follows the parameter as the fp32 layer does, and no later eager call can free what it reads.
             packed = dense_ops.fp8_weight(w.detach(), gain=self.weight_gain)
         else:
             src, made_for, packed = getattr(self, "_fp8", (None, None, None))

@@ -183,3 +183,17 @@ def test_image_follows_a_new_parameter_on_the_same_memory(dev):
     layer.weight.data.mul_(0.5)
     layer._fp8 = (None, None, None)
     assert torch.equal(layer.forward_fp8(q, s), want())
+
+
+@pytest.mark.gpu
+def test_weights_without_versions(dev):
+    """Parameters made under inference_mode track no versions: no image is kept of them, and the layer works as the fp32 one does."""
+    from nerffaceediting_amd.training.networks_stylegan2 import MappingNetwork
+    with torch.inference_mode():
+        layer, q, s, want = make(dev)
+        assert torch.equal(layer.forward_fp8(q, s), want())
+        layer.weight.mul_(2.0)
+        assert torch.equal(layer.forward_fp8(q, s), want())
+        m = MappingNetwork(128, 25, 128, 4, num_layers=2, embed_features=128, fc_math="fp8").to(dev)
+        assert m(torch.randn(3, 128, device=dev), torch.randn(3, 25, device=dev)).shape == (3, 4, 128)
+    assert torch.equal(layer.forward_fp8(q, s), want())
