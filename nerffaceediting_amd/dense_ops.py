@@ -20,7 +20,7 @@ def nchw_to_nhwc(x):
     lib = _lib.load()
     x = _dev(x, "x", (None, None, None, None))
     N, C, H, W = x.shape
-    out = torch.empty(N, H, W, C, device=x.device)
+    out = torch.empty(N, H, W, C, dtype=torch.float32, device=x.device)
     _call(x.device, lambda: lib.nfe_nchw_to_nhwc(_ptr(x), N, C, H, W, _ptr(out), _stream()), "nfe_nchw_to_nhwc")
     return out
 
@@ -31,7 +31,7 @@ def nhwc_to_nchw(x):
     lib = _lib.load()
     x = _dev(x, "x", (None, None, None, None))
     N, H, W, C = x.shape
-    out = torch.empty(N, C, H, W, device=x.device)
+    out = torch.empty(N, C, H, W, dtype=torch.float32, device=x.device)
     _call(x.device, lambda: lib.nfe_nhwc_to_nchw(_ptr(x), N, C, H, W, _ptr(out), _stream()), "nfe_nhwc_to_nchw")
     return out
 
@@ -41,7 +41,7 @@ def nhwc_to_planes(x):
     lib = _lib.load()
     x = _dev(x, "planes", (None, None, None, 96))
     N, H, W, _ = x.shape
-    out = torch.empty(N, 3, H, W, 32, device=x.device)
+    out = torch.empty(N, 3, H, W, 32, dtype=torch.float32, device=x.device)
     _call(x.device, lambda: lib.nfe_nhwc_to_planes(_ptr(x), N, H, W, _ptr(out), _stream()), "nfe_nhwc_to_planes")
     return out
 
@@ -51,7 +51,7 @@ def plane_stats_nhwc(x):
     lib = _lib.load()
     x = _dev(x, "planes", (None, None, None, None))
     N, H, W, C = x.shape
-    mean = torch.empty(N, C, 1, 1, device=x.device)
+    mean = torch.empty(N, C, 1, 1, dtype=torch.float32, device=x.device)
     std = torch.empty_like(mean)
     scratch = torch.empty(N * C * 2, dtype=torch.float64, device=x.device)
     _call(x.device, lambda: lib.nfe_plane_stats_nhwc(_ptr(x), N, H * W, C, _ptr(mean), _ptr(std), _ptr(scratch), _stream()),
@@ -69,7 +69,7 @@ def fully_connected(x, weight, bias, weight_gain, bias_gain=1.0, lrelu=False, ou
     if bias is not None:
         bias = _dev(bias, "bias", (fout,))
     if out is None:
-        out = torch.empty(N, fout, device=x.device)
+        out = torch.empty(N, fout, dtype=torch.float32, device=x.device)
         view, stride = out, fout
     else:
         stride = out.shape[1]
@@ -90,7 +90,7 @@ def fully_connected_grouped(groups):
     for i, (x, w, b, wg, bg) in enumerate(groups):
         assert x.is_cuda and x.dtype == torch.float32 and x.dim() == 2 and x.shape[0] == N and x.stride(1) == 1
         w = _dev(w, "weight", (None, x.shape[1]))
-        y = torch.empty(N, w.shape[0], device=dev)
+        y = torch.empty(N, w.shape[0], dtype=torch.float32, device=dev)
         g = arr[i]
         g.x, g.x_stride, g.w, g.b, g.y = x.data_ptr(), x.stride(0) if N > 1 else x.shape[1], w.data_ptr(), (b.data_ptr() if b is not None else None), y.data_ptr()
         g.in_features, g.out_features, g.weight_gain, g.bias_gain = x.shape[1], w.shape[0], float(wg), float(bg)
@@ -107,7 +107,7 @@ def conv_demod_grouped(pairs, prenormalize=False):
     N, dev = pairs[0][0].shape[0], pairs[0][0].device
     outs, norms = [], []
     for i, (s, wsq) in enumerate(pairs):
-        d = torch.empty(N, wsq.shape[0], device=dev)
+        d = torch.empty(N, wsq.shape[0], dtype=torch.float32, device=dev)
         g = arr[i]
         g.styles, g.wsq, g.dcoef, g.cin, g.cout = s.data_ptr(), wsq.data_ptr(), d.data_ptr(), s.shape[1], wsq.shape[0]
         if prenormalize:
@@ -140,7 +140,7 @@ def broadcast_truncate(w, w_avg, num_ws, psi=1.0, cutoff=None):
     if w_avg is not None:
         w_avg = _dev(w_avg, "w_avg", (D,))
     cutoff = num_ws if cutoff is None else int(cutoff)
-    ws = torch.empty(N, num_ws, D, device=w.device)
+    ws = torch.empty(N, num_ws, D, dtype=torch.float32, device=w.device)
     _call(w.device, lambda: lib.nfe_broadcast_truncate(_ptr(w), _ptr(w_avg), N, D, num_ws, float(psi), cutoff, _ptr(ws), _stream()),
           "nfe_broadcast_truncate")
     return ws
@@ -158,8 +158,8 @@ def conv_pack(weight, math=None, prenormalize=False):
         raise RuntimeError(f"conv_pack: unsupported weight shape {list(weight.shape)}")
     f16 = MATH[math] == _lib.NFE_CONV_F16
     assert f16 or not prenormalize, "prenormalize belongs to the fp16 operand mode"
-    packed = torch.empty(words + (cout if f16 else 0), device=weight.device)
-    wsq = torch.empty(cout, cin, device=weight.device)
+    packed = torch.empty(words + (cout if f16 else 0), dtype=torch.float32, device=weight.device)
+    wsq = torch.empty(cout, cin, dtype=torch.float32, device=weight.device)
     if f16:
         _call(weight.device, lambda: lib.nfe_conv_pack_f16(_ptr(weight), cout, cin, k, int(bool(prenormalize)), _ptr(packed), _ptr(wsq), _stream()),
               "nfe_conv_pack_f16")
@@ -176,7 +176,7 @@ def conv_demod(styles, wsq, prenormalize=False):
     N, cin = styles.shape
     wsq = _dev(wsq, "wsq", (None, cin))
     cout = wsq.shape[0]
-    d = torch.empty(N, cout, device=styles.device)
+    d = torch.empty(N, cout, dtype=torch.float32, device=styles.device)
     sn = torch.empty_like(styles) if prenormalize else None
     _call(styles.device, lambda: lib.nfe_conv_demod(_ptr(styles), _ptr(wsq), N, cin, cout, _ptr(d), _ptr(sn), _stream()), "nfe_conv_demod")
     return (d, sn) if prenormalize else d
@@ -267,24 +267,24 @@ def modulated_conv(x, styles, packed, cout, mode, bias, dcoef=None, noise=None, 
         rw, rs, rb, rskip, rclamp = rgb
         C = rw.shape[0]
         rw = _dev(rw.reshape(C, cout), "rgb_weight", (C, cout)); rs = _dev(rs, "rgb_styles", (N, cout)); rb = _dev(rb, "rgb_bias", (C,))
-        rgb_out = torch.empty(N, Ho, Wo, C, device=dev)
+        rgb_out = torch.empty(N, Ho, Wo, C, dtype=torch.float32, device=dev)
         a.rgb_weight, a.rgb_styles, a.rgb_bias, a.rgb_out, a.rgb_channels = rw.data_ptr(), rs.data_ptr(), rb.data_ptr(), rgb_out.data_ptr(), C
         a.rgb_clamp = -1.0 if rclamp is None else float(rclamp)
         if rskip is not None:
             rskip = _dev(rskip, "rgb_skip", (N, H // 2, W // 2, C)); a.rgb_skip = rskip.data_ptr()
         keep += [rw, rs, rb, rskip, rgb_out]
     if want_out or (next_styles is None and rgb is None):
-        out = torch.empty((N, 3, Ho, Wo, 32) if out_planes else (N, Ho, Wo, cout), device=dev)
+        out = torch.empty((N, 3, Ho, Wo, 32) if out_planes else (N, Ho, Wo, cout), dtype=torch.float32, device=dev)
         a.out = out.data_ptr()
     split = None
     if next_styles is not None:
         next_styles = _dev(next_styles, "next_styles", (N, cout))
-        split = SplitImage(torch.empty(int(lib.nfe_conv_split_floats(a.math, N, Ho, Wo, cout)), device=dev), (N, Ho, Wo, cout), a.math)
+        split = SplitImage(torch.empty(int(lib.nfe_conv_split_floats(a.math, N, Ho, Wo, cout)), dtype=torch.float32, device=dev), (N, Ho, Wo, cout), a.math)
         a.next_styles, a.next_split = next_styles.data_ptr(), split.data.data_ptr()
     scratch = None
     n_scratch = int(lib.nfe_conv_scratch_floats(a.mode, a.math, N, H, W, cin, cout)) if FAST_PATH else (N * (2 * H + 1) * (2 * W + 1) * cout if up == 2 else 0)
     if n_scratch:                    # up-conv intermediate, or the pre-split input image of the 3x3 fast path
-        scratch = torch.empty(n_scratch, device=dev)
+        scratch = torch.empty(n_scratch, dtype=torch.float32, device=dev)
         a.scratch, a.scratch_floats = scratch.data_ptr(), n_scratch
     keep += [dcoef, noise, bias, skip, scratch, next_styles, split]
     _call(dev, lambda: lib.nfe_modulated_conv(ctypes.byref(a), _stream()), "nfe_modulated_conv")
@@ -300,7 +300,7 @@ def upfirdn2d(x, up=1, down=1, padding=(0, 0), gain=1.0):
     N, H, W, C = x.shape
     p0, p1 = int(padding[0]), int(padding[1])
     oh, ow = (H * up + p0 + p1 - 4) // down + 1, (W * up + p0 + p1 - 4) // down + 1
-    out = torch.empty(N, oh, ow, C, device=x.device)
+    out = torch.empty(N, oh, ow, C, dtype=torch.float32, device=x.device)
     _call(x.device, lambda: lib.nfe_upfirdn2d(_ptr(x), N, H, W, C, int(up), int(down), p0, p1, float(gain), _ptr(out), _stream()), "nfe_upfirdn2d")
     return out
 
@@ -315,7 +315,7 @@ def resize_bilinear_backward(g, h, w, antialias=True):
     lib = _lib.load()
     g = _dev(g, "g", (None, None, None, None))
     N, OH, OW, C = g.shape
-    out = torch.empty(N, int(h), int(w), C, device=g.device)
+    out = torch.empty(N, int(h), int(w), C, dtype=torch.float32, device=g.device)
     _call(g.device, lambda: lib.nfe_resize_bilinear_backward(_ptr(g), N, int(h), int(w), C, OH, OW, int(bool(antialias)), _ptr(out), _stream()),
           "nfe_resize_bilinear_backward")
     return out
@@ -328,7 +328,7 @@ def upfirdn2d_polyphase(x, padding=(2, 2), gain=1.0):
     x = _dev(x, "x", (None, None, None, None))
     N, H, W, C = x.shape
     OH, OW = H + padding[0] + padding[1] - 3, W + padding[0] + padding[1] - 3
-    out = torch.empty(N, (OH + 1) // 2, (OW + 1) // 2, 4 * C, device=x.device)
+    out = torch.empty(N, (OH + 1) // 2, (OW + 1) // 2, 4 * C, dtype=torch.float32, device=x.device)
     _call(x.device, lambda: lib.nfe_upfirdn2d_polyphase(_ptr(x), N, H, W, C, int(padding[0]), int(padding[1]), float(gain), _ptr(out), _stream()),
           "nfe_upfirdn2d_polyphase")
     return out
@@ -364,7 +364,7 @@ def resize_bilinear(x, oh, ow, antialias=True):
     lib = _lib.load()
     x = _dev(x, "x", (None, None, None, None))
     N, H, W, C = x.shape
-    out = torch.empty(N, oh, ow, C, device=x.device)
+    out = torch.empty(N, oh, ow, C, dtype=torch.float32, device=x.device)
     _call(x.device, lambda: lib.nfe_resize_bilinear(_ptr(x), N, H, W, C, int(oh), int(ow), int(bool(antialias)), _ptr(out), _stream()),
           "nfe_resize_bilinear")
     return out
@@ -417,7 +417,7 @@ def _fp8_out(what, out, out_offset, rows, cols, dev):
     if out is None:
         if out_offset:
             raise ValueError(f"{what}: out_offset needs out")
-        return torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=dev), torch.empty_strided((rows, blocks), (1, rows), device=dev)
+        return torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=dev), torch.empty_strided((rows, blocks), (1, rows), dtype=torch.float32, device=dev)
     q, scale = out
     b = out_offset // FP8_BLOCK
     if out_offset % FP8_BLOCK or out_offset < 0 or q.dtype != torch.float8_e4m3fn or q.dim() != 2 or not q.is_contiguous() or q.shape[0] != rows or \
@@ -497,7 +497,7 @@ def fp8_weight(weight, gain=1.0):
     weight = _fp8_rows(weight, "weight").detach()
     n, k = weight.shape
     packed = _fp8_weight_buffer(lib, n, k, weight.device)
-    scale = torch.empty(_fp8_blocks(n), _fp8_blocks(k), device=weight.device)
+    scale = torch.empty(_fp8_blocks(n), _fp8_blocks(k), dtype=torch.float32, device=weight.device)
     _call(weight.device, lambda: lib.nfe_fp8_weight_quantize(_ptr(weight), _FP8_TYPES[weight.dtype], n, k, float(gain), _ptr(packed), _ptr(scale), _stream()),
           "nfe_fp8_weight_quantize")
     return Fp8Weight(packed, scale, n, k)

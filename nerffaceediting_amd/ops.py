@@ -139,7 +139,7 @@ def ray_sampler(cam2world, intrinsics, resolution):
     N = cam2world.shape[0]
     intrinsics = _dev(intrinsics, "intrinsics", (N, 3, 3))
     R = int(resolution)
-    o = torch.empty(N, R * R, 3, device=cam2world.device)
+    o = torch.empty(N, R * R, 3, dtype=torch.float32, device=cam2world.device)
     d = torch.empty_like(o)
     with torch.cuda.device(cam2world.device):
         _lib.check(lib.nfe_ray_sampler(_ptr(cam2world), _ptr(intrinsics), N, R, _ptr(o), _ptr(d), _stream()), "nfe_ray_sampler")
@@ -152,7 +152,7 @@ def ray_limits_box(origins, dirs, box_side_length):
     origins = _dev(origins, "ray_origins", (None, None, 3))
     dirs = _dev(dirs, "ray_directions", tuple(origins.shape))
     N, M = origins.shape[:2]
-    rs = torch.empty(N, M, 1, device=origins.device)
+    rs = torch.empty(N, M, 1, dtype=torch.float32, device=origins.device)
     re = torch.empty_like(rs)
     scratch = torch.empty(2, dtype=torch.int32, device=origins.device)
     with torch.cuda.device(origins.device):
@@ -166,7 +166,7 @@ def plane_stats(planes):
     lib = _lib.load()
     planes = _dev(planes, "planes", (None, None, None, None))
     N, C, H, W = planes.shape
-    mean = torch.empty(N, C, 1, 1, device=planes.device)
+    mean = torch.empty(N, C, 1, 1, dtype=torch.float32, device=planes.device)
     std = torch.empty_like(mean)
     with torch.cuda.device(planes.device):
         _lib.check(lib.nfe_plane_stats(_ptr(planes), N, C, H * W, _ptr(mean), _ptr(std), _stream()), "nfe_plane_stats")
@@ -202,7 +202,7 @@ def make_affine(mean, std, new_mean=None, new_std=None):
         new_std = _dev(new_std, "planes_var").reshape(-1, C)
         no = new_mean.shape[0]
         assert new_std.shape[0] == no and no in (1, N), "override statistics must be [N,C,1,1] or [1,C,1,1]"
-    outs = [torch.empty(N, C, device=mean.device) for _ in range(4)]
+    outs = [torch.empty(N, C, dtype=torch.float32, device=mean.device) for _ in range(4)]
     with torch.cuda.device(mean.device):
         _lib.check(lib.nfe_make_affine(_ptr(mean), _ptr(std), _ptr(new_mean), _ptr(new_std), N, C, no,
                                        *[_ptr(o) for o in outs], _stream()), "nfe_make_affine")
@@ -216,7 +216,7 @@ def plane_pack(planes):
         planes = planes.reshape(planes.shape[0], 96, planes.shape[-2], planes.shape[-1])
     planes = _dev(planes, "planes", (None, 96, None, None))
     N, _, H, W = planes.shape
-    out = torch.empty(N, 3, H, W, 32, device=planes.device)
+    out = torch.empty(N, 3, H, W, 32, dtype=torch.float32, device=planes.device)
     with torch.cuda.device(planes.device):
         _lib.check(lib.nfe_plane_pack(_ptr(planes), N, H, W, _ptr(out), _stream()), "nfe_plane_pack")
     return out
@@ -228,7 +228,7 @@ def decoder_pack(geo_w0, geo_b0, geo_w1, geo_b1, app_w0, app_b0, app_w1, app_b1,
           _dev(geo_w1, "geo_net.2.weight", (16, 64)), _dev(geo_b1, "geo_net.2.bias", (16,)),
           _dev(app_w0, "app_net.0.weight", (64, 32)), _dev(app_b0, "app_net.0.bias", (64,)),
           _dev(app_w1, "app_net.2.weight", (32, 64)), _dev(app_b1, "app_net.2.bias", (32,))]
-    out = torch.empty(_lib.NFE_DECODER_PACKED_FLOATS, device=ts[0].device)
+    out = torch.empty(_lib.NFE_DECODER_PACKED_FLOATS, dtype=torch.float32, device=ts[0].device)
     with torch.cuda.device(out.device):
         _lib.check(lib.nfe_decoder_pack(*[_ptr(t) for t in ts], float(lr_mul), _ptr(out), _stream()), "nfe_decoder_pack")
     return out
@@ -238,7 +238,7 @@ def decoder_pack_cross(cross_w1, lr_mul=1.0):
     """nfe_decoder_pack_cross: [16,64] geometry-head rows on the appearance head's hidden units (SegmentationOSGDecoder)."""
     lib = _lib.load()
     cross_w1 = _dev(cross_w1, "cross_w1", (16, 64))
-    out = torch.empty(_lib.NFE_DECODER_CROSS_FLOATS, device=cross_w1.device)
+    out = torch.empty(_lib.NFE_DECODER_CROSS_FLOATS, dtype=torch.float32, device=cross_w1.device)
     with torch.cuda.device(out.device):
         _lib.check(lib.nfe_decoder_pack_cross(_ptr(cross_w1), float(lr_mul), _ptr(out), _stream()), "nfe_decoder_pack_cross")
     return out
@@ -255,9 +255,9 @@ def decoder_forward(features_geo, features_app, decoder_packed, decoder_math=Non
     decoder_packed = _dev(decoder_packed, "decoder_packed", (_lib.NFE_DECODER_PACKED_FLOATS,))
     if decoder_cross is not None:
         decoder_cross = _dev(decoder_cross, "decoder_cross", (_lib.NFE_DECODER_CROSS_FLOATS,))
-    rgb = torch.empty(N, P, 32, device=dev)
-    sigma = torch.empty(N, P, 1, device=dev)
-    seg = torch.empty(N, P, 15, device=dev)
+    rgb = torch.empty(N, P, 32, dtype=torch.float32, device=dev)
+    sigma = torch.empty(N, P, 1, dtype=torch.float32, device=dev)
+    seg = torch.empty(N, P, 15, dtype=torch.float32, device=dev)
     if N * P > 0:
         with torch.cuda.device(dev):
             _lib.check(lib.nfe_decoder_forward(_ptr(features_geo), _ptr(features_app), N, n_planes, P, _ptr(decoder_packed),
@@ -353,25 +353,25 @@ def render(planes_geo, planes_app, decoder_packed, options, *, origins=None, dir
         keep.append(seed)
     else:
         a.seed = int(seed) & 0xFFFFFFFFFFFFFFFF
-    rgb = torch.empty((N, 32, M) if channels_first else (N, M, 32), device=dev)
-    seg = torch.empty((N, 15, M) if channels_first else (N, M, 15), device=dev)
-    depth = torch.empty(N, M, 1, device=dev)
-    wsum = torch.empty(N, M, 1, device=dev)
+    rgb = torch.empty((N, 32, M) if channels_first else (N, M, 32), dtype=torch.float32, device=dev)
+    seg = torch.empty((N, 15, M) if channels_first else (N, M, 15), dtype=torch.float32, device=dev)
+    depth = torch.empty(N, M, 1, dtype=torch.float32, device=dev)
+    wsum = torch.empty(N, M, 1, dtype=torch.float32, device=dev)
     a.rgb, a.seg, a.depth, a.wsum = rgb.data_ptr(), seg.data_ptr(), depth.data_ptr(), wsum.data_ptr()
     a.channels_first = int(channels_first)
     tap = {}
     if taps:
-        tap["depths_all"] = torch.empty(N, M, D + Di, device=dev)
+        tap["depths_all"] = torch.empty(N, M, D + Di, dtype=torch.float32, device=dev)
         a.tap_depths_all = tap["depths_all"].data_ptr()
         if Di > 0:
-            tap["weights_coarse"] = torch.empty(N, M, D - 1, device=dev)
-            tap["depths_fine"] = torch.empty(N, M, Di, device=dev)
+            tap["weights_coarse"] = torch.empty(N, M, D - 1, dtype=torch.float32, device=dev)
+            tap["depths_fine"] = torch.empty(N, M, Di, dtype=torch.float32, device=dev)
             a.tap_weights_coarse, a.tap_depths_fine = tap["weights_coarse"].data_ptr(), tap["depths_fine"].data_ptr()
         if sample_colors:
             # the decoders' outputs for every sample of the final march (192 bytes per sample, opaque): render_backward(...,
             # sample_colors=) then skips its re-evaluation pass.  Split-bf16 decoder without density noise / cross decoder only.
             assert a.decoder_math == _lib.NFE_MATH_BF16X3, "sample_colors needs the split-bf16 decoder"
-            tap["sample_colors"] = torch.empty(lib.nfe_render_sample_colors_floats(N, M, D + Di), device=dev)
+            tap["sample_colors"] = torch.empty(lib.nfe_render_sample_colors_floats(N, M, D + Di), dtype=torch.float32, device=dev)
             a.tap_sample_colors = tap["sample_colors"].data_ptr()
             # the buffer's ray order follows the launch's ray-block shape (8x4 pixel tiles when resolution % 8 == 0 and resolution^2 ==
             # n_rays, else 32 consecutive rays): render_backward must be given the same `resolution` and checks it against this
@@ -497,9 +497,9 @@ def point_query(planes_geo, planes_app, decoder_packed, coords, box_warp, affine
     if affines is not None:
         aff = [_dev(t, "affine", (N, 96)) for t in affines]
     decoder_packed = _dev(decoder_packed, "decoder_packed", (_lib.NFE_DECODER_PACKED_FLOATS,))
-    rgb = torch.empty(N, P, 32, device=dev)
-    sigma = torch.empty(N, P, 1, device=dev)
-    seg = torch.empty(N, P, 15, device=dev)
+    rgb = torch.empty(N, P, 32, dtype=torch.float32, device=dev)
+    sigma = torch.empty(N, P, 1, dtype=torch.float32, device=dev)
+    seg = torch.empty(N, P, 15, dtype=torch.float32, device=dev)
     if P == 0:                                   # empty query: nothing to launch (zero-size tensors have no storage)
         return {"rgb": rgb, "sigma": sigma, "seg": seg}
     stride = 0 if (Np == 1 and N > 1) else 3 * H * W * 32
@@ -571,7 +571,7 @@ def _grad_call(what, tensors, norm_type, max_norm=None):
     types = (ctypes.c_int32 * n).from_buffer(array("i", types))
     with _on(index):
         dev = ts[0].device
-        norm = torch.empty((), device=dev)
+        norm = torch.empty((), dtype=torch.float32, device=dev)
         # partial sums of this call alone: _workspace begins with the render calls' status words, and a call from another host thread may
         # put its launches between this one's
         ws = torch.empty(lib.nfe_grad_workspace_bytes(n), dtype=torch.uint8, device=dev)

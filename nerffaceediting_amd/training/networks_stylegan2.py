@@ -121,7 +121,7 @@ class MappingNetwork(torch.nn.Module):
         if self.fc_math == "fp8":
             x = self._layers_fp8(z.detach().to(torch.float32), c)
             return dense_ops.broadcast_truncate(x, self.w_avg if psi != 1 else None, self.num_ws, psi, cutoff)
-        buf = torch.empty(N, self.z_dim + self.embed_features, device=z.device)
+        buf = torch.empty(N, self.z_dim + self.embed_features, dtype=torch.float32, device=z.device)
         dense_ops.normalize_2nd_moment(z.to(torch.float32), out=buf, out_offset=0)                 # :240
         if self.c_dim > 0:
             assert c.shape[1] == self.c_dim, f"Wrong size for dimension 1: got {c.shape[1]}, expected {self.c_dim}"
@@ -136,7 +136,7 @@ class MappingNetwork(torch.nn.Module):
         """The norms (:240, :244) and the layers on 8-bit operands; the camera's embedding (25 inputs) stays fp32."""
         N, width = z.shape[0], self.z_dim + self.embed_features
         q = torch.empty(N, width, dtype=torch.float8_e4m3fn, device=z.device)
-        scale = torch.empty(width // dense_ops.FP8_BLOCK, N, device=z.device).t()
+        scale = torch.empty(width // dense_ops.FP8_BLOCK, N, dtype=torch.float32, device=z.device).t()
         dense_ops.rms_norm_fp8(z, out=(q, scale))
         if self.c_dim > 0:
             assert c.shape[1] == self.c_dim, f"Wrong size for dimension 1: got {c.shape[1]}, expected {self.c_dim}"
