@@ -549,7 +549,7 @@ def fp8_matmul(q, scale, weight, bias=None, bias_gain=1.0, lrelu=False, out_dtyp
         return out
     stride, inner = q.stride()
     if inner != 1 or q.data_ptr() % 16 or (N > 1 and (stride % 16 or stride < width)):
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)      # contiguous() would return a contiguous q at an odd address as it is
         stride = width
     a = _lib.Fp8MatmulArgs(_FP8_MATMUL_ARGS, N, n, k, q.data_ptr(), stride if N > 1 else width, scale.data_ptr(), scale.stride(0), scale.stride(1),
                            weight.packed.data_ptr(), weight.scale.data_ptr(), _address(bias), bias_gain, 1 if lrelu else 0, _FP8_TYPES[out_dtype],

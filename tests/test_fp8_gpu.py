@@ -493,3 +493,18 @@ def test_many_rows_and_wide_strides(dev):
     got = dense_ops.fp8_matmul(wide.view(torch.float8_e4m3fn), ss.to(dev), W)
     want, mag = mm64(qs, ss, wq, ws, dev)
     check_mm(got, want, mag, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 7])
+def test_rows_at_any_address(dev, rows):
+    """Contiguous rows that begin anywhere (a view into a byte buffer) are copied where the kernel needs 16-byte alignment."""
+    from nerffaceediting_amd import dense_ops
+    q, s, wq, ws = make_mm(rows, 40, 300)
+    W = dense_ops.fp8_weight_from(wq.to(dev), ws.to(dev))
+    want = dense_ops.fp8_matmul(q.to(dev), s.to(dev), W)
+    for start in (1, 8, 15, 16):
+        flat = torch.full((start + q.numel() + 16,), 0x7F, dtype=torch.uint8, device=dev)
+        view = flat[start:start + q.numel()].view(q.shape)
+        view.copy_(q.view(torch.uint8))
+        assert torch.equal(dense_ops.fp8_matmul(view.view(torch.float8_e4m3fn), s.to(dev), W), want), start
