@@ -380,9 +380,19 @@ def _fp8_blocks(n):
     return -(-n // FP8_BLOCK)
 
 
+# what the library takes; a larger number must not reach it, as its 32-bit arguments would hold the low bits alone
+_FP8_ROWS, _FP8_COLS, _FP8_OUT, _FP8_MATMUL_ROWS = (1 << 31) - 1, 1 << 30, 65535 * FP8_BLOCK, 1 << 30
+
+
+def _fp8_size(name, t, rows, cols):
+    if t.shape[0] > rows or t.shape[1] > cols:
+        raise ValueError(f"{name}: {list(t.shape)} is too large, at most [{rows}, {cols}]")
+
+
 def _fp8_rows(t, name, like=None):
     """_dev for the types the 8-bit operators read: a contiguous GPU matrix (of like's shape and type)."""
     if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _FP8_TYPES and t.dim() == 2 and (like is None or (t.shape == like.shape and t.dtype == like.dtype)):
+        _fp8_size(name, t, _FP8_ROWS, _FP8_COLS)
         return t.contiguous()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor, got {type(t)}")
@@ -494,6 +504,8 @@ def fp8_weight(weight, gain=1.0):
     """nfe_fp8_weight_quantize: weight [out, in] (fp32 / bf16 / fp16), rounded to e4m3 with one scale for every 128 x 128 block; gain
     multiplies the scales (FullyConnectedLayer's weight_gain).  A NaN or an infinity makes its whole block NaN."""
     lib = _lib.load()
+    if isinstance(weight, torch.Tensor) and weight.dim() == 2:
+        _fp8_size("weight", weight, _FP8_OUT, _FP8_COLS)
     weight = _fp8_rows(weight, "weight").detach()
     n, k = weight.shape
     packed = _fp8_weight_buffer(lib, n, k, weight.device)
@@ -510,6 +522,7 @@ def fp8_weight_from(q, scale):
         raise RuntimeError("fp8_weight_from: q must be a float8_e4m3fn tensor [out, in]")
     if q.device.type != "cuda":
         raise RuntimeError(f"fp8_weight_from: q is on {q.device}; this path runs only on the GPU (no CPU fallback)")
+    _fp8_size("q", q, _FP8_OUT, _FP8_COLS)
     q = q.contiguous()
     n, k = q.shape
     scale = _dev(scale, "scale", (_fp8_blocks(n), _fp8_blocks(k)))
@@ -539,6 +552,7 @@ def fp8_matmul(q, scale, weight, bias=None, bias_gain=1.0, lrelu=False, out_dtyp
     width = kb * FP8_BLOCK
     assert q.dim() == 2 and q.shape[1] == width, \
         f"q: wrong shape {list(q.shape)}, expected [N, {width}] ({k} input features in blocks of {FP8_BLOCK})"
+    _fp8_size("q", q, _FP8_MATMUL_ROWS, width)
     N = q.shape[0]
     if not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or scale.shape != (N, kb):
         raise RuntimeError(f"fp8_matmul: scale must be a float32 tensor [{N}, {kb}]")

@@ -508,3 +508,27 @@ def test_rows_at_any_address(dev, rows):
         view = flat[start:start + q.numel()].view(q.shape)
         view.copy_(q.view(torch.uint8))
         assert torch.equal(dense_ops.fp8_matmul(view.view(torch.float8_e4m3fn), s.to(dev), W), want), start
+
+
+@pytest.mark.gpu
+def test_sizes_beyond_the_library_are_refused(dev):
+    """Widths that a 32-bit argument would take for smaller ones: refused before anything is copied or allocated (expanded rows hold one value)."""
+    from nerffaceediting_amd import dense_ops
+    one = torch.ones(1, 1, device=dev, dtype=torch.bfloat16)
+    free = torch.cuda.mem_get_info(dev)[0]
+    for cols in ((1 << 30) + 1, (1 << 32) + 1):
+        wide = one.expand(1, cols)
+        for call in (lambda: dense_ops.quantize_fp8(wide), lambda: dense_ops.rms_norm_fp8(wide), lambda: dense_ops.rms_norm_fp8(wide, residual=wide),
+                     lambda: dense_ops.fp8_weight(wide), lambda: dense_ops.fp8_weight(wide.t()),
+                     lambda: dense_ops.fp8_weight_from(one.to(torch.float8_e4m3fn).expand(1, cols), torch.ones(1, 1, device=dev))):
+            with pytest.raises(ValueError, match="at most"):
+                call()
+    for rows in (1 << 31, (1 << 32) + 1):
+        with pytest.raises(ValueError, match="at most"):
+            dense_ops.quantize_fp8(one.expand(rows, 1))
+    W = dense_ops.fp8_weight(torch.ones(3, 5, device=dev))
+    rows = (1 << 30) + 1
+    q = torch.zeros(1, 128, device=dev).to(torch.float8_e4m3fn).expand(rows, 128)
+    with pytest.raises(ValueError, match="at most"):
+        dense_ops.fp8_matmul(q, torch.ones(1, 1, device=dev).expand(rows, 1), W)
+    assert free - torch.cuda.mem_get_info(dev)[0] < 1 << 30
