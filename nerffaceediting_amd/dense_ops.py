@@ -480,7 +480,16 @@ class Fp8Weight:
     """e4m3 weights [out_features, in_features] in fp8_matmul's operand order, with their scales [ceil(out / 128), ceil(in / 128)]."""
 
     def __init__(self, packed, scale, out_features, in_features):
-        self.packed, self.scale, self.out_features, self.in_features = packed, scale, int(out_features), int(in_features)
+        n, k = int(out_features), int(in_features)
+        if not isinstance(packed, torch.Tensor) or not isinstance(scale, torch.Tensor):
+            raise TypeError(f"Fp8Weight: expected torch.Tensors, got {type(packed)} and {type(scale)}")
+        size = -(-n // 16) * _fp8_blocks(k) * 16 * FP8_BLOCK                 # nfe_fp8_weight_bytes
+        if n <= 0 or k <= 0 or packed.dtype != torch.uint8 or packed.numel() != size or not packed.is_contiguous() or \
+                scale.dtype != torch.float32 or tuple(scale.shape) != (_fp8_blocks(n), _fp8_blocks(k)) or not scale.is_contiguous() or \
+                scale.device != packed.device:
+            raise ValueError(f"Fp8Weight: [{n}, {k}] needs packed uint8 [{size}] and scale float32 [{_fp8_blocks(n)}, {_fp8_blocks(k)}], both contiguous "
+                             "and on one device")
+        self.packed, self.scale, self.out_features, self.in_features = packed, scale, n, k
         self._stream = self._current_stream()
 
     def _current_stream(self):

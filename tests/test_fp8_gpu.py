@@ -532,3 +532,16 @@ def test_sizes_beyond_the_library_are_refused(dev):
     with pytest.raises(ValueError, match="at most"):
         dense_ops.fp8_matmul(q, torch.ones(1, 1, device=dev).expand(rows, 1), W)
     assert free - torch.cuda.mem_get_info(dev)[0] < 1 << 30
+
+
+def test_weight_objects_are_checked_when_made():
+    """Fp8Weight's sizes say how far the kernel reads: buffers that do not hold them are refused."""
+    from nerffaceediting_amd.dense_ops import Fp8Weight
+    packed, scale = torch.zeros(3 * 2 * 2048, dtype=torch.uint8), torch.ones(1, 2)
+    assert Fp8Weight(packed, scale, 33, 200).in_features == 200
+    for bad in ((packed, scale, 49, 200), (packed, scale, 32, 200), (packed, scale, 33, 257), (packed[1:], scale, 33, 200), (packed.float(), scale, 33, 200),
+                (packed, scale[:, :1], 33, 200), (packed, scale.double(), 33, 200), (packed, torch.ones(2, 2)[:, :1].expand(2, 2)[:1], 33, 200),
+                (packed, torch.ones(1, 4)[:, ::2], 33, 200), (torch.zeros(2 * packed.numel(), dtype=torch.uint8)[::2], scale, 33, 200),
+                (packed, scale, 0, 200), (packed, scale, 33, -200), (packed.tolist(), scale, 33, 200)):
+        with pytest.raises((ValueError, TypeError), match="Fp8Weight"):
+            Fp8Weight(*bad)
