@@ -222,7 +222,7 @@ int nfe_grad_clip(const uint64_t* data, const int64_t* n, const int32_t* dtype, 
 
 /* ---- 8-bit rows: e4m3 values (OCP, largest 448) with one fp32 scale for every 128 columns (ABI v16) ----------------------------
  *   h = x + residual                      (residual NULL: h = x)
- *   y = h * rsqrt(mean(h^2) + eps) * weight   (nfe_rms_norm_fp8; weight NULL: ones; networks_stylegan2.py:24-26 with weight NULL, eps 1e-8)
+ *   y = h * rsqrt(mean(h^2) + eps) * weight   (nfe_rms_norm_fp8; eps >= 2^-126; weight NULL: ones; networks_stylegan2.py:24-26 with weight NULL, eps 1e-8)
  *   y = x                                 (nfe_quantize_fp8)
  *   per 128 columns: a = max(max |y|, 1e-30), scale = a / 448, q = e4m3(y / scale), round to nearest even
  * x, residual, h: [rows, cols] of `dtype`, contiguous; h (required with residual, and only then) gets x + residual rounded to `dtype` - the

@@ -719,7 +719,7 @@ static int norm_entry(const char* who, NormArgs& a, int dtype, bool norm, nfe_st
     NFE_REQUIRE((a.residual != nullptr) == (a.h != nullptr), "%s: residual and h come in pairs", who);
     const int width = (a.cols + BLOCK - 1) / BLOCK * BLOCK;
     NFE_REQUIRE(a.q_stride >= width && a.q_stride % 8 == 0 && (uintptr_t)a.q % 8 == 0, "%s: q rows must be 8-byte aligned and at least %d bytes apart", who, width);
-    NFE_REQUIRE(!norm || a.eps > 0.0f, "%s: eps must be positive", who);
+    NFE_REQUIRE(!norm || a.eps >= 1.17549435e-38f, "%s: eps must be a positive normal number", who);      // v_rsq_f32 takes less for zero
     const long long rows = a.rows, most = 1 << 22;                    // 2^32 work items are a launch's limit
     for (long long at = 0; at < rows; at += most) {
         NormArgs part = a;

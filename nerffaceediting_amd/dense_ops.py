@@ -450,8 +450,8 @@ def rms_norm_fp8(x, weight=None, residual=None, eps=1e-8, out=None, out_offset=0
     residual = _fp8_rows(residual, "residual", x) if residual is not None else None
     weight = _dev(weight, "weight", (K,)) if weight is not None else None
     index = _fp8_check("rms_norm_fp8", x, residual, weight)
-    if K == 0 or not eps > 0:
-        raise ValueError("rms_norm_fp8: rows need at least one column and eps must be positive")
+    if K == 0 or not eps >= 2.0 ** -126:
+        raise ValueError("rms_norm_fp8: rows need at least one column and eps must be a positive normal number (2^-126 at least)")
     q, scale = _fp8_out("rms_norm_fp8", out, out_offset, N, K, x.device)
     h = torch.empty_like(x) if residual is not None else None
     if N:

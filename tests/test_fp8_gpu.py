@@ -545,3 +545,23 @@ def test_weight_objects_are_checked_when_made():
                 (packed, scale, 0, 200), (packed, scale, 33, -200), (packed.tolist(), scale, 33, 200)):
         with pytest.raises((ValueError, TypeError), match="Fp8Weight"):
             Fp8Weight(*bad)
+
+
+@pytest.mark.gpu
+def test_smallest_eps(dev):
+    """The reciprocal root's instruction takes subnormal numbers for zero: eps is at least the smallest normal number, and works there."""
+    from nerffaceediting_amd import dense_ops
+    x = torch.zeros(3, 200, device=dev)
+    x[1] = 2.0 ** -70
+    q, s = dense_ops.rms_norm_fp8(x, eps=2.0 ** -126)
+    check_rows(q, s, norm64(x, None, None, eps=2.0 ** -126)[0], 200)
+    for eps in (2.0 ** -127, 1e-40, 1e-50):
+        with pytest.raises(ValueError, match="eps"):
+            dense_ops.rms_norm_fp8(x, eps=eps)
+
+
+def test_smallest_eps_of_the_library():
+    from nerffaceediting_amd import _lib
+    lib = _lib.load()
+    for eps in (2.0 ** -127, 1e-45, float("nan")):
+        assert lib.nfe_rms_norm_fp8(64, None, None, 0, 2, 200, eps, None, 4096, 256, 64, 1, 2, None) == -1 and b"eps" in lib.nfe_last_error()
