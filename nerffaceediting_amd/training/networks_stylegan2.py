@@ -85,6 +85,8 @@ class MappingNetwork(torch.nn.Module):
     features of a row and every 128 x 128 block of a weight, fp32 sums): for large batches of latents; w differs from the fp32 path's by
     the operands' rounding (about 3 % of its own size)."""
 
+    fc_math = None                     # of networks pickled before there was a choice
+
     def __init__(self, z_dim, c_dim, w_dim, num_ws, num_layers=8, embed_features=None, layer_features=None,
                  activation="lrelu", lr_multiplier=0.01, w_avg_beta=0.998, fc_math=None):
         super().__init__()

@@ -197,3 +197,14 @@ def test_weights_without_versions(dev):
         m = MappingNetwork(128, 25, 128, 4, num_layers=2, embed_features=128, fc_math="fp8").to(dev)
         assert m(torch.randn(3, 128, device=dev), torch.randn(3, 25, device=dev)).shape == (3, 4, 128)
     assert torch.equal(layer.forward_fp8(q, s), want())
+
+
+def test_mapping_networks_saved_before_fc_math():
+    """A module pickled when MappingNetwork had no fc_math loads as the fp32 network that it was."""
+    from nerffaceediting_amd.training.networks_stylegan2 import MappingNetwork
+    m = MappingNetwork(16, 4, 16, 2, num_layers=2)
+    del m.__dict__["fc_math"]
+    file = io.BytesIO()
+    torch.save(m, file)
+    file.seek(0)
+    assert torch.load(file, weights_only=False).fc_math is None
