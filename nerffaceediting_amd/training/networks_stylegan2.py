@@ -100,6 +100,8 @@ class MappingNetwork(torch.nn.Module):
             raise ValueError(f"unknown fc_math {fc_math!r}")
         if fc_math == "fp8" and (z_dim % dense_ops.FP8_BLOCK or embed_features % dense_ops.FP8_BLOCK):
             raise ValueError(f"fc_math='fp8' needs z_dim ({z_dim}) and embed_features ({embed_features}) in multiples of {dense_ops.FP8_BLOCK}")
+        if fc_math == "fp8" and num_layers < 1:
+            raise ValueError(f"fc_math='fp8' needs num_layers ({num_layers}) of at least 1")
         self.fc_math = fc_math
         if layer_features is None:
             layer_features = w_dim

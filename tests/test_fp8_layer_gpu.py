@@ -208,3 +208,10 @@ def test_mapping_networks_saved_before_fc_math():
     torch.save(m, file)
     file.seek(0)
     assert torch.load(file, weights_only=False).fc_math is None
+
+
+def test_fp8_stack_without_layers_is_refused():
+    from nerffaceediting_amd.training.networks_stylegan2 import MappingNetwork
+    with pytest.raises(ValueError, match="num_layers"):
+        MappingNetwork(128, 0, 128, 4, num_layers=0, fc_math="fp8")
+    assert MappingNetwork(128, 0, 128, 4, num_layers=0).num_layers == 0
