@@ -643,10 +643,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_tile_kernel(MatmulArgs
     block_sync();
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
+        if (p > 0) wave_sync();                          // other lanes still read the part before
 #pragma unroll
         for (int i = 0; i < PM; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j) *(f32x4*)(mine + ((i * 16 + r) * CHUNKS + ((j * 4 + g) ^ (r & (CHUNKS - 1)))) * 16) = acc[p * PM + i][j];
+        wave_sync();
         finish<WIDE>(A, f, [&](auto store) {
 #pragma unroll 4
             for (int t = 0; t < PM * NT; ++t) {

@@ -45,6 +45,12 @@ __device__ __forceinline__ float wave_sum(float v) {
     const auto b = __builtin_amdgcn_permlane32_swap(bits_of(v), bits_of(v), false, false);      // (lower half twice, upper half twice)
     return float_of(b[0]) + float_of(b[1]);
 }
+// LDS accesses of one wave: those before it come first, for every lane.  An order for the compiler, no instruction.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 __device__ __forceinline__ void block_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
     __builtin_amdgcn_s_barrier();
