@@ -261,6 +261,8 @@ typedef struct nfe_fp8_matmul_args {
     void* out;
 } nfe_fp8_matmul_args;
 int nfe_fp8_matmul(const nfe_fp8_matmul_args* args, nfe_stream_t stream);
+/* Diagnostic text: which kernel nfe_fp8_matmul runs for these sizes and strides on the current device (ABI v17). */
+int nfe_fp8_matmul_describe(int m, int n, int64_t q_stride, int64_t scale_row_stride, int out_dtype, char* buf, int buf_len);
 
 #ifdef __cplusplus
 }

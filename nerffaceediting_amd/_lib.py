@@ -7,7 +7,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # NFE_RENDER_LIB lets tools/ load an experimental build of the same ABI (kernel ablations)
 LIB_PATH = os.environ.get("NFE_RENDER_LIB") or os.path.join(_HERE, "libnfe_render.so")
 
-NFE_ABI_VERSION = 16
+NFE_ABI_VERSION = 17
 NFE_MAX_SAMPLES = 256
 NFE_DECODER_PACKED_FLOATS = 4 * 2048 + 64 + 64 + 32 + 32 + 8192
 NFE_DECODER_CROSS_FLOATS = 2048
@@ -162,6 +162,7 @@ _SIGNATURES = {
     "nfe_fp8_weight_quantize": (c_int, [FP, c_int, c_int, c_int, c_float, FP, FP, c_void_p]),
     "nfe_fp8_weight_pack": (c_int, [FP, c_int, c_int, FP, c_void_p]),
     "nfe_fp8_matmul": (c_int, [POINTER(Fp8MatmulArgs), c_void_p]),
+    "nfe_fp8_matmul_describe": (c_int, [c_int, c_int, c_int64, c_int64, c_int, c_char_p, c_int]),
     "nfe_point_query": (c_int, [FP, FP, c_int, c_int, c_int64, FP, FP, FP, FP, FP, c_int, FP, c_int, c_int, c_float,
                                 FP, FP, FP, c_float, c_uint64, FP, c_void_p]),
 }

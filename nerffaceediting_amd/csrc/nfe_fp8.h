@@ -2,6 +2,7 @@
 // product of the two.  Part of nfe_dense.hip's code object, beside the fp32 fully-connected layers they are the 8-bit form of.
 #pragma once
 #include <algorithm>
+#include <cstdio>
 
 #include "nfe_dense.h"
 #include "nfe_wave.h"
@@ -688,25 +689,34 @@ static int rows_launch(const MatmulArgs& A, hipStream_t st) {
 //   128 x 256 tile                       1.94             1.94   4096^3: 124
 // E.g. 10000 x 512 x 1024 fp32: 64 x 64 5 rounds x 0.36, 128 x 128 2 x 1.15, 128 x 256 1 x 1.94: 18.5, 24.5, 21.8 us measured.
 // Offsets inside a tile are 32-bit: 256 rows of up to 2^23 bytes (and scales that far apart); anything wider stays on the rows kernels.
-template <bool WIDE>
-static int matmul_launch(const MatmulArgs& A, hipStream_t st) {
+enum Choice { ROWS_16X16, ROWS_16X32, ROWS_32X32, ROWS_32X64, TILE_64X64, TILE_128X128, TILE_LARGE };
+static Choice choose(bool wide, int m, int n, long long a_stride, long long scale_row) {
     const int cus = num_cus();
-    auto count = [&](int bm, int bn) { return (((long long)A.m + bm - 1) / bm) * (((long long)A.n + bn - 1) / bn); };
-    const bool near = A.a_stride <= (1 << 23) && A.scale_row <= (1 << 21);
-    if (A.m <= 16) return count(16, 32) < cus ? rows_launch<WIDE, 1, 1, 8>(A, st) : rows_launch<WIDE, 1, 2, 8>(A, st);
-    if (count(32, 64) < cus || !near) {
-        if (count(32, 32) < cus && near) return count(16, 32) < cus ? rows_launch<WIDE, 1, 1, 8>(A, st) : rows_launch<WIDE, 1, 2, 8>(A, st);
-        if (near) return rows_launch<WIDE, 2, 2, 8>(A, st);
-        return rows_launch<WIDE, 2, 4, 4>(A, st);
+    auto count = [&](int bm, int bn) { return (((long long)m + bm - 1) / bm) * (((long long)n + bn - 1) / bn); };
+    const bool near = a_stride <= (1 << 23) && scale_row <= (1 << 21);
+    if (m <= 16) return count(16, 32) < cus ? ROWS_16X16 : ROWS_16X32;
+    if (!near) return ROWS_32X64;
+    if (count(32, 64) < cus) {
+        if (count(32, 32) < cus) return count(16, 32) < cus ? ROWS_16X16 : ROWS_16X32;
+        return ROWS_32X32;
     }
     auto cost = [&](int bm, int bn, double full, double alone) { return std::max(alone, full * (double)((count(bm, bn) + cus - 1) / cus)); };
-    const double rows = WIDE ? cost(32, 64, 0.28, 0.33) : cost(32, 64, 0.23, 0.29), small = WIDE ? cost(64, 64, 0.36, 0.67) : cost(64, 64, 0.30, 0.62),
-                 middle = WIDE ? cost(128, 128, 1.15, 1.20) : cost(128, 128, 0.66, 0.82), large = WIDE ? cost(128, 256, 1.94, 1.94) : cost(256, 256, 2.0, 2.0);
+    const double rows = wide ? cost(32, 64, 0.28, 0.33) : cost(32, 64, 0.23, 0.29), small = wide ? cost(64, 64, 0.36, 0.67) : cost(64, 64, 0.30, 0.62),
+                 middle = wide ? cost(128, 128, 1.15, 1.20) : cost(128, 128, 0.66, 0.82), large = wide ? cost(128, 256, 1.94, 1.94) : cost(256, 256, 2.0, 2.0);
     const double best = std::min(std::min(rows, small), std::min(middle, large));
-    if (rows == best) return rows_launch<WIDE, 2, 4, 4>(A, st);
-    if (small == best) return tile_launch<WIDE, 2, 2, 2, 2>(A, st);
-    if (middle == best) return tile_launch<WIDE, 2, 4, 4, 2>(A, st);
-    return WIDE ? tile_launch<true, 2, 4, 4, 4>(A, st) : tile_launch<false, 2, 4, 8, 4>(A, st);
+    return rows == best ? ROWS_32X64 : small == best ? TILE_64X64 : middle == best ? TILE_128X128 : TILE_LARGE;
+}
+template <bool WIDE>
+static int matmul_launch(const MatmulArgs& A, hipStream_t st) {
+    switch (choose(WIDE, A.m, A.n, A.a_stride, A.scale_row)) {
+        case ROWS_16X16: return rows_launch<WIDE, 1, 1, 8>(A, st);
+        case ROWS_16X32: return rows_launch<WIDE, 1, 2, 8>(A, st);
+        case ROWS_32X32: return rows_launch<WIDE, 2, 2, 8>(A, st);
+        case ROWS_32X64: return rows_launch<WIDE, 2, 4, 4>(A, st);
+        case TILE_64X64: return tile_launch<WIDE, 2, 2, 2, 2>(A, st);
+        case TILE_128X128: return tile_launch<WIDE, 2, 4, 4, 2>(A, st);
+        default: return WIDE ? tile_launch<true, 2, 4, 4, 4>(A, st) : tile_launch<false, 2, 4, 8, 4>(A, st);
+    }
 }
 
 static int check_rows(const char* who, long long rows, int cols) {
@@ -799,5 +809,16 @@ extern "C" int nfe_fp8_matmul(const nfe_fp8_matmul_args* p, nfe_stream_t stream)
                  p->scale_block_stride, p->m, p->n, kblocks, p->lrelu, p->out_dtype, p->bias_gain};
     if (int rc = p->out_dtype == NFE_F32 ? matmul_launch<true>(A, (hipStream_t)stream) : matmul_launch<false>(A, (hipStream_t)stream)) return rc;
     NFE_CHECK_LAUNCH("nfe_fp8_matmul");
+    return NFE_OK;
+}
+extern "C" int nfe_fp8_matmul_describe(int m, int n, int64_t q_stride, int64_t scale_row_stride, int out_dtype, char* buf, int buf_len) {
+    using namespace nfe::fp8;
+    NFE_REQUIRE(buf && buf_len > 0, "nfe_fp8_matmul_describe: no buffer");
+    NFE_REQUIRE(m > 0 && n > 0, "nfe_fp8_matmul_describe: bad sizes m=%d n=%d", m, n);
+    NFE_REQUIRE(out_dtype == NFE_F32 || out_dtype == NFE_BF16 || out_dtype == NFE_F16, "nfe_fp8_matmul_describe: unknown out_dtype %d", out_dtype);
+    static const char* names[] = {"rows 16x16/8w", "rows 16x32/8w", "rows 32x32/8w", "rows 32x64/4w", "tile 64x64/4w", "tile 128x128/8w"};
+    const bool wide = out_dtype == NFE_F32;
+    const Choice c = choose(wide, m, n, q_stride, scale_row_stride);
+    snprintf(buf, (size_t)buf_len, "%s %s", c != TILE_LARGE ? names[c] : wide ? "tile 128x256/8w" : "tile 256x256/8w", wide ? "widened" : "8-bit");
     return NFE_OK;
 }

@@ -580,3 +580,10 @@ def fp8_matmul(q, scale, weight, bias=None, bias_gain=1.0, lrelu=False, out_dtyp
     with _on(index):
         _lib.check(_lib.load().nfe_fp8_matmul(ctypes.byref(a), _stream()), "nfe_fp8_matmul")
     return out
+
+
+def describe_fp8_matmul(m, n, out_dtype=torch.float32, q_stride=FP8_BLOCK, scale_row_stride=1):
+    """nfe_fp8_matmul_describe: which kernel fp8_matmul runs for m rows and n outputs (diagnostic text)."""
+    buf = ctypes.create_string_buffer(64)
+    _lib.check(_lib.load().nfe_fp8_matmul_describe(int(m), int(n), int(q_stride), int(scale_row_stride), _FP8_TYPES[out_dtype], buf, 64), "nfe_fp8_matmul_describe")
+    return buf.value.decode()
