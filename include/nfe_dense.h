@@ -228,8 +228,9 @@ int nfe_grad_clip(const uint64_t* data, const int64_t* n, const int32_t* dtype, 
  * x, residual, h: [rows, cols] of `dtype`, contiguous; h (required with residual, and only then) gets x + residual rounded to `dtype` - the
  * norm uses the sum before that rounding.  weight: [cols] fp32.  q: [rows][q_stride] bytes, q_stride >= cols rounded up to 128 and a multiple
  * of 8; columns from `cols` up to that width are written as zeros.  scale of row r, block b: scale[r * scale_row_stride + b *
- * scale_block_stride] (block-major, scale_row_stride = 1, is what nfe_fp8_matmul reads fastest).  A NaN or an infinity makes every value
- * of its block read as NaN.  Sums and products are fp32. */
+ * scale_block_stride] (block-major, scale_row_stride = 1, is what nfe_fp8_matmul reads fastest).  A block that holds a NaN or an infinity
+ * reads as NaN in all its values.  In nfe_rms_norm_fp8 a NaN reaches its whole row through the mean, an infinity makes the row's other blocks
+ * zeros, and so does a sum of squares beyond fp32 for all of its row.  Sums and products are fp32. */
 int nfe_rms_norm_fp8(const void* x, const void* residual, const float* weight, int dtype, int64_t rows, int cols, float eps, void* h, void* q,
                      int64_t q_stride, float* scale, int64_t scale_row_stride, int64_t scale_block_stride, nfe_stream_t stream);
 int nfe_quantize_fp8(const void* x, int dtype, int64_t rows, int cols, void* q, int64_t q_stride, float* scale, int64_t scale_row_stride,

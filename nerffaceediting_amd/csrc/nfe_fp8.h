@@ -53,7 +53,8 @@ __device__ __forceinline__ unsigned e4m3x4(float a, float b, float c, float d) {
 // h = x + residual;  y = h * rsqrt(mean(h^2) + eps) * weight  (NORM) or y = h;  then per 128 columns
 //   a = max(max |y|, 1e-30),  scale = a / 448,  q = e4m3(y / scale)
 // Everything between the load of x and the rounding to e4m3 (and of h to x's type) is fp32.  The maximum is taken on the bits, so a NaN or
-// an infinity in a block makes its scale NaN or infinite and every value of the block reads as NaN.
+// an infinity in a block of y makes its scale NaN or infinite and every value of the block reads as NaN.  With the norm a NaN in h is in every
+// block of y, and an infinity makes 1 / sqrt(mean) zero: NaN in its own block, zeros in the others.
 // One row belongs to WAVES waves; a lane holds 8 neighbouring columns of every step, so 16 lanes share a scale.  STEPS > 0: the row stays
 // in registers and is read once; STEPS = 0: longer rows, read twice.
 // Bound by memory where the rows fill the chip: 16384 x 4096 bf16 with a residual (472 MB) 89.6 us = 5.27 TB/s, a large copy's rate.  A few

@@ -444,6 +444,7 @@ def rms_norm_fp8(x, weight=None, residual=None, eps=1e-8, out=None, out_offset=0
     """nfe_rms_norm_fp8: h = x + residual; y = h * rsqrt(mean(h^2) + eps) * weight, rounded to e4m3 with one fp32 scale for every 128 columns.
     x [N,K] fp32 / bf16 / fp16, residual like x, weight [K] fp32.  Returns (q [N, Kp] float8_e4m3fn, scale [N, Kp / 128] fp32) - Kp is K
     rounded up to 128, the columns from K on are zero - and with a residual also h [N,K] in x's type.  y ~ q * scale per block.
+    A NaN in a row makes the row NaN; an infinity makes its own block NaN and the row's other blocks zero.
     out = (q, scale) buffers and out_offset (columns, a multiple of 128) write into wider rows.  Inference only."""
     x = _fp8_rows(x, "x")
     N, K = x.shape
@@ -462,7 +463,8 @@ def rms_norm_fp8(x, weight=None, residual=None, eps=1e-8, out=None, out_offset=0
 
 
 def quantize_fp8(x, out=None, out_offset=0):
-    """nfe_quantize_fp8: rms_norm_fp8 without the norm (the operand of the next layer's fp8_matmul) -> (q, scale)."""
+    """nfe_quantize_fp8: rms_norm_fp8 without the norm (the operand of the next layer's fp8_matmul) -> (q, scale).  A NaN or an
+    infinity makes its block of 128 columns NaN."""
     x = _fp8_rows(x, "x")
     N, K = x.shape
     index = _fp8_check("quantize_fp8", x)

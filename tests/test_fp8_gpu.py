@@ -565,3 +565,30 @@ def test_smallest_eps_of_the_library():
     lib = _lib.load()
     for eps in (2.0 ** -127, 1e-45, float("nan")):
         assert lib.nfe_rms_norm_fp8(64, None, None, 0, 2, 200, eps, None, 4096, 256, 64, 1, 2, None) == -1 and b"eps" in lib.nfe_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [384, 700, 5000])
+def test_special_values_in_the_norm(dev, cols):
+    """The formula's: a NaN makes the mean and so its whole row NaN; an infinity makes its own block NaN (infinity times zero) and the row's
+    other blocks zero; squares whose sum leaves fp32 make the row zero; a NaN weight makes its block of every row NaN."""
+    from nerffaceediting_amd import dense_ops
+    x = torch.ones(6, cols, device=dev)
+    x[1, 200], x[2, 5], x[3, cols - 1] = float("inf"), float("nan"), -float("inf")
+    x[4] = 1e25
+    q, scale = dense_ops.rms_norm_fp8(x)
+    bad = torch.isnan(q.float().view(6, -1, BLOCK) * scale[..., None]).cpu()
+    want = torch.zeros(6, blocks(cols), dtype=torch.bool)
+    want[1, 1], want[2], want[3, blocks(cols) - 1] = True, True, True
+    assert torch.equal(bad.all(-1), want) and torch.equal(bad.any(-1), want)
+    value = (q.float().view(6, -1, BLOCK) * scale[..., None]).cpu()
+    for row in (1, 3):
+        assert not bool(value[row][~want[row]].any())
+    assert not bool(value[4].any()) and bool(torch.isfinite(scale[4]).all())
+    for row in (0, 5):
+        check_rows(q[row:row + 1], scale[row:row + 1], norm64(x[row:row + 1].cpu(), None, None)[0], cols)
+    weight = torch.ones(cols, device=dev)
+    weight[130] = float("nan")
+    q, scale = dense_ops.rms_norm_fp8(x[:1], weight)
+    bad = torch.isnan(q.float().view(-1, BLOCK) * scale[0][:, None])
+    assert bool(bad[1].all()) and not bool(bad[0].any()) and not bool(bad[2:].any())
