@@ -19,7 +19,6 @@ __device__ __forceinline__ float float_of(unsigned b) { return __builtin_bit_cas
 __device__ __forceinline__ int wave_lane() { return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
 // the value of lane (own ^ off); every lane of the wave has to take part
 __device__ __forceinline__ unsigned wave_xor(unsigned v, int off) { return (unsigned)__builtin_amdgcn_ds_bpermute((wave_lane() ^ off) << 2, (int)v); }
-__device__ __forceinline__ float wave_xor(float v, int off) { return float_of(wave_xor(bits_of(v), off)); }
 __device__ __forceinline__ double wave_xor(double v, int off) {
     const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
     const unsigned lo = wave_xor((unsigned)b, off), hi = wave_xor((unsigned)(b >> 32), off);
