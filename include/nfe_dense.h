@@ -248,7 +248,9 @@ int nfe_fp8_weight_pack(const void* q, int n, int k, void* packed, nfe_stream_t 
  * out[i, o] = act( sum_b scale[i, b] w_scale[o / 128, b] sum_{c in block b} q[i, c] w[o, c]  +  bias[o] * bias_gain ),
  * act = linear or lrelu(0.2) * sqrt(2); block sums are scaled and added in fp32 and rounded once to out_dtype.  A block's sum over its 128
  * columns is fp32-grade for NFE_F32 outputs (e4m3 widened to bf16 operands, exact products); for NFE_BF16 / NFE_F16 outputs it is the
- * 8-bit matrix instruction's, off by less than 7 2^-13 sum|products| (1.5e-5 of the result for normally distributed operands).
+ * 8-bit matrix instruction's, off by less than 7 2^-13 sum|products| (1.5e-5 of the result for normally distributed operands; more than the
+ * result's own rounding where products cancel: a 16-bit result of exact sums is an NFE_F32 result, rounded).  The two scales' product is formed
+ * first and must be a normal fp32 number (or the block's sum zero).
  * q: [m][q_stride] bytes, 16-byte aligned rows, ceil(k/128)*128 columns (those from k on must be zero or meet zero weights: any finite
  * value).  out: [m, n] contiguous. */
 typedef struct nfe_fp8_matmul_args {

@@ -59,7 +59,8 @@ __device__ __forceinline__ unsigned e4m3x4(float a, float b, float c, float d) {
 // in registers and is read once; STEPS = 0: longer rows, read twice.
 // Bound by memory where the rows fill the chip: 16384 x 4096 bf16 with a residual (472 MB) 89.6 us = 5.27 TB/s, a large copy's rate.  A few
 // thousand short rows are one round of waves and cost its latency: 10001 x 1031 fp16 (31 MB) 11.5 us.  Asking for a row's weights before its
-// values, or for the next row's values early, took registers and won nothing.
+// values, or for the next row's values early, took registers and won nothing.  Without the norm 10000 x 512 fp32 (26 MB) takes 3.9 us on the GPU
+// (4.4 with it), 16384 x 4096 bf16 (203 MB, in part from cache) 33 us (34); a call takes 9 us at least.
 // ------------------------------------------------------------------------------------------------
 struct NormArgs {
     const void* x; const void* residual; const float* weight; void* h;
@@ -242,6 +243,7 @@ static void norm_dispatch(const NormArgs& a, bool norm, hipStream_t st) {
 // columns 64 h + 16 (l / 16) .. + 15 of row l % 16, so a fragment is two contiguous kilobytes.  (The instruction sums over all 128
 // columns, whose order is free as long as both operands share it.)  Rows and columns beyond n and k are zero.
 // Runs once for a set of weights, so it is plain: a workgroup reads its 128 x 128 block twice (the second time from cache) and stores bytes.
+// 512 x 1024 fp32 25 us, 4096 x 4096 54 us, 8192 x 8192 (335 MB) 146 us.
 // ------------------------------------------------------------------------------------------------
 __device__ __forceinline__ long long packed_at(int n, int k, int kblocks) {
     const int c = k & 127;
@@ -290,7 +292,8 @@ __global__ __launch_bounds__(256) void weight_fp8_kernel(const void* w, const un
 //   FP8 (bf16 and fp16 outputs): one v_mfma_f32_16x16x128_f8f6f4.  The unit adds eight products at a time in fixed point, at 2^-13 of the
 //     power of two of the largest (measured: next to one product of 2^16, products below 2^3 vanish if they are among its eight and count
 //     to 2^-7 otherwise; truncated towards zero), so a sum is off by less than 7 2^-13 sum|products| - 1.5e-5 of its size for normally
-//     distributed values, an eighth of the rounding to fp16 and a hundredth of that to bf16;
+//     distributed values, an eighth of the rounding to fp16 and a hundredth of that to bf16.  Where products cancel, that bound is far above
+//     the result's own rounding: a 16-bit result of exact sums is the fp32 output and a cast;
 //   WIDE (fp32 output): both operands widened to bf16, which holds every e4m3 value, and four v_mfma_f32_16x16x32_bf16: exact products,
 //     fp32 sums, half the rate.
 // The weights are the instruction's first operand: lane l then holds outputs 4 (l / 16) .. + 3 of row l % 16, whose scale is one number
@@ -389,7 +392,7 @@ template <bool WIDE, typename F> __device__ __forceinline__ void finish(const Ma
 // Few rows, or few tiles.  A workgroup of WAVES waves owns 16 MT rows x 16 NT columns; its waves share the K blocks, read both operands straight
 // into registers, one block ahead, and join their sums through LDS in the order of the waves.  Bound by reading: every weight once for each 16 MT
 // rows, every row once for each 16 NT columns.  16 x 8192 x 8192 (67.5 MB, in part from cache) 12.2 us, a library product with one scale in place of
-// the blocks' 20.2; 1 x 512 x 1024 2.8 us on the GPU, little more than an empty launch.
+// the blocks' 20.2; 1 x 512 x 1024 2.3 us in a replayed graph (2.9 in a trace), little more than an empty launch.
 template <bool WIDE, int MT, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, MT * NT >= 8 ? 2 : MT * NT >= 4 ? 3 : 4) void matmul_rows_kernel(MatmulArgs A) {
     __shared__ f32x4 part[WAVES][MT * NT][64];
@@ -487,7 +490,8 @@ __global__ __launch_bounds__(64 * WAVES, MT * NT >= 8 ? 2 : MT * NT >= 4 ? 3 : 4
 // quarter into it, the weights of kb + 1.  The one barrier, in the middle of the block, says that the rows of kb + 1 are there for everybody, so no wave stops
 // between blocks; and as nobody is left in block kb - 2 then, buffer (kb + 2) % 4 is free when block kb begins.
 // Workgroups b, b + 8, .. run on one XCD: each XCD gets a contiguous range of tiles, GROUP row tiles deep, so that its L2 serves both operands.
-// 4096^3 bf16 62 us = 2200 TFLOP/s (a library product with one scale 2730), 8191 x 8190 x 8192 fp16 470 us = 2340 (3106).  The matrix unit is busy 0.53
+// 4096^3 bf16 63 us = 2190 TFLOP/s (a library product with one scale 2730), 8191 x 8190 x 8192 fp16 462 - 477 us = 2300 - 2380 (3106): a call in a
+// row of calls; the medians of a kernel trace lie above, 68 and 529 us.  The matrix unit is busy 0.53
 // (4096^3) and 0.62 (8192^3) of the time, a third of a wave's life is waiting, there are no LDS conflicts, and the vector unit's scaling runs under
 // the products (16.4 ns for an instruction with its four additions, 15.4 without): what is left is the waits for L2 at a block's start.
 // LDS-DMA: 64 lanes x 16 (4) bytes from base + offset into 1 KiB (256 bytes) at dst.  Inline assembly, because the compiler would wait for the DMA
@@ -681,14 +685,15 @@ static int rows_launch(const MatmulArgs& A, hipStream_t st) {
 // outputs: 16 x 16384 x 4096 15.9 -> 12.7 us, 16 x 20000 x 8192 32.7 -> 27.1, 1 x 65536 x 2048 22.4 -> 21.1; bf16 13.9 -> 12.6, 31.1 -> 26.8, 21.9 -> 21.1).
 // More: rows kernels: the largest tile that still gives every CU a workgroup (their waves share K, so a short chain of blocks stays
 // short).  Among the widest of them and the tile kernels: the least of rounds x (time of one workgroup's K block), rounds = workgroups /
-// CUs rounded up, but not less than what a lone workgroup takes for a block (loads' latency).  us measured on 256 CUs, K block = 128:
+// CUs rounded up, but not less than what a lone workgroup takes for a block (loads' latency).  The times are of 256 CUs and one clock; another number
+// of CUs is counted, but its choice has not been measured.  us, K block = 128; "measured": a call in a row of calls on the same operands
 //                       a workgroup's block, CU full   alone     measured
-//   32 x 64   rows   8-bit 0.23, widened 0.28       0.29, 0.33   128 x 8192 x 8192: 29.5 (bf16), 31.3 us (fp32); 64 rows: 18.6, 20.9
-//   64 x 64   tile         0.30          0.36       0.62, 0.67   512 x 4096 x 4096: 21.7, 27.6
-//   128 x 128 tile         0.66          1.15       0.82, 1.20   2048^3: 15.0, 22.8
-//   256 x 256 tile         2.00                     2.00         4096^3: 67
-//   128 x 256 tile                       1.94             1.94   4096^3: 124
-// E.g. 10000 x 512 x 1024 fp32: 64 x 64 5 rounds x 0.36, 128 x 128 2 x 1.15, 128 x 256 1 x 1.94: 18.5, 24.5, 21.8 us measured.
+//   32 x 64   rows   8-bit 0.23, widened 0.28       0.29, 0.33   128 x 8192 x 8192: 26.5 (bf16), 28.6 us (fp32); 64 rows: 16.0, 19.8
+//   64 x 64   tile         0.30          0.36       0.62, 0.67   512 x 4096 x 4096: 16.8, 25.0
+//   128 x 128 tile         0.66          1.15       0.82, 1.20   2048^3: 12.7, 21.2
+//   256 x 256 tile         2.00                     2.00         4096^3: 63
+//   128 x 256 tile                       1.94             1.94   4096^3: 118
+// E.g. 10000 x 512 x 1024 fp32: 64 x 64 5 rounds x 0.36, 128 x 128 2 x 1.15, 128 x 256 1 x 1.94: 17.4 - 18.5, 24.5, 21.8 us measured.
 // Offsets inside a tile are 32-bit: 256 rows of up to 2^23 bytes (and scales that far apart); anything wider stays on the rows kernels.
 enum Choice { ROWS_16X16, ROWS_16X32, ROWS_32X32, ROWS_32X64, TILE_64X64, TILE_128X128, TILE_LARGE };
 static Choice choose(bool wide, int m, int n, long long a_stride, long long scale_row) {

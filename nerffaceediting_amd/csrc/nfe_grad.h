@@ -3,7 +3,7 @@
 //
 //   t = sqrt(sum_i sum_j g_ij^2)   (or max |g_ij|),   f = min(1, max_norm / (t + 1e-6)),   g_ij <- round(f g_ij)
 //
-// Two launches for up to TABLE tensors: grad_reduce_kernel leaves one fp64 partial per workgroup, grad_clip_kernel adds the
+// Two launches for up to TABLE tensors (for more, two for each TABLE, of which each scaling one adds the partials of all): grad_reduce_kernel leaves one fp64 partial per workgroup, grad_clip_kernel adds the
 // partials in their order in every workgroup (no atomics: the same call gives the same bits) and scales.  Nothing is read or written a
 // second time when f = 1.  Both are bound by memory: 50.3 million fp32 values (201 MB) take 48.6 + 65.9 us, three passes at the 5.3 TB/s of a
 // large copy; 6.3 million that need no clipping 6.8 + 4.5 us.  (Clipping from the last chunk back, to find it in the last-level cache, changed

@@ -548,8 +548,10 @@ def fp8_matmul(q, scale, weight, bias=None, bias_gain=1.0, lrelu=False, out_dtyp
     """nfe_fp8_matmul: FullyConnectedLayer.forward on the 8-bit rows of rms_norm_fp8 / quantize_fp8 and an Fp8Weight:
     act( (q * scale) @ (w * w_scale).T + bias * bias_gain ), act = linear or lrelu(0.2) * sqrt(2), rounded once to out_dtype -> [N, out].
     out_dtype fp32 sums exact products in fp32; bf16 and fp16 use the 8-bit matrix instructions at twice the rate, whose sums over a block
-    are off by less than 7 2^-13 sum|products| (typically 1.5e-5 of the result, below the output's own rounding).  q [N, Kp] float8_e4m3fn with Kp = in_features rounded up to 128 (zeros, or any finite values, from
-    in_features on), scale [N, Kp / 128] fp32 of any strides (block-major, as rms_norm_fp8 returns it, is read fastest).  Inference only."""
+    are off by less than 7 2^-13 sum|products|: typically 1.5e-5 of the result, below the output's own rounding, but above it where the
+    products cancel.  A 16-bit result of exact sums is out_dtype=torch.float32 and a cast.
+    q [N, Kp] float8_e4m3fn with Kp = in_features rounded up to 128 (zeros, or any finite values, from in_features on), scale [N, Kp / 128]
+    fp32 of any strides (block-major, as rms_norm_fp8 returns it, is read fastest).  Inference only."""
     if not isinstance(weight, Fp8Weight):
         raise TypeError(f"fp8_matmul: weight must be an Fp8Weight (fp8_weight, fp8_weight_from), got {type(weight)}")
     if not isinstance(q, torch.Tensor) or q.dtype != torch.float8_e4m3fn:

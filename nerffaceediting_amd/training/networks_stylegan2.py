@@ -83,7 +83,8 @@ class FullyConnectedLayer(torch.nn.Module):
 class MappingNetwork(torch.nn.Module):
     """networks_stylegan2.py:193-271.  fc_math='fp8' runs the fully-connected stack on e4m3 operands (one scale for every 128 input
     features of a row and every 128 x 128 block of a weight, fp32 sums): for large batches of latents; w differs from the fp32 path's by
-    the operands' rounding (about 3 % of its own size)."""
+    the operands' rounding (about 3 % of its own size).  Two layers of 512, 14 w each, us a call (fp32 path, fp8): 1 and 64 latents 63, 84;
+    1000 643, 110; 10000 6250, 900.  A captured call rounds the weights at every replay, 25 us a layer: 1000 latents 177."""
 
     fc_math = None                     # of networks pickled before there was a choice
 
