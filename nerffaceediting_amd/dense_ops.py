@@ -59,6 +59,15 @@ def plane_stats_nhwc(x):
     return mean, std
 
 
+def _wide_rows(what, out, out_offset, rows, cols, dev):
+    """(view, row stride) of columns out_offset .. of the caller's buffer, which has to hold rows x cols there."""
+    if out.dtype != torch.float32 or out.dim() != 2 or not out.is_contiguous() or out.device != dev or out.shape[0] != rows or \
+            out_offset < 0 or out.shape[1] < out_offset + cols:
+        raise ValueError(f"{what}: out must be float32 [{rows}, S] on {dev}, contiguous, with {cols} columns from out_offset {out_offset}; got {out.dtype} "
+                         f"{list(out.shape)} on {out.device}")
+    return out[:, out_offset:], out.shape[1]
+
+
 def fully_connected(x, weight, bias, weight_gain, bias_gain=1.0, lrelu=False, out=None, out_offset=0):
     """FullyConnectedLayer.forward; `out` (a [N,S] buffer) + out_offset write into a wider row (concat)."""
     lib = _lib.load()
@@ -72,8 +81,7 @@ def fully_connected(x, weight, bias, weight_gain, bias_gain=1.0, lrelu=False, ou
         out = torch.empty(N, fout, dtype=torch.float32, device=x.device)
         view, stride = out, fout
     else:
-        stride = out.shape[1]
-        view = out[:, out_offset:]
+        view, stride = _wide_rows("fully_connected", out, out_offset, N, fout, x.device)
     _call(x.device, lambda: lib.nfe_fully_connected(_ptr(x), _ptr(weight), _ptr(bias), N, fin, fout, float(weight_gain),
                                                     float(bias_gain), int(bool(lrelu)),
                                                     ctypes.c_void_p(view.data_ptr()), stride, _stream()), "nfe_fully_connected")
@@ -126,8 +134,7 @@ def normalize_2nd_moment(x, out=None, out_offset=0):
         out = torch.empty_like(x)
         view, stride = out, f
     else:
-        stride = out.shape[1]
-        view = out[:, out_offset:]
+        view, stride = _wide_rows("normalize_2nd_moment", out, out_offset, N, f, x.device)
     _call(x.device, lambda: lib.nfe_normalize_2nd_moment(_ptr(x), N, f, ctypes.c_void_p(view.data_ptr()), stride, _stream()),
           "nfe_normalize_2nd_moment")
     return out
