@@ -163,6 +163,25 @@ def test_long_sums(dev, m, n, k):
         check(dense_ops.fp8_matmul(q.to(dev), s.to(dev), W, out_dtype=dtype), want, mag, k)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["tile 256x256/8w 8-bit", "tile 128x256/8w widened"])
+def test_widest_strides_of_a_tile(dev, name):
+    """Rows 2^23 bytes and scales 2^21 values apart, the most that the tiles' 32-bit offsets take: 255 rows are 2^31 - 2^23 bytes."""
+    from nerffaceediting_amd import dense_ops
+    dtype = torch.float32 if "widened" in name else torch.bfloat16
+    k, (m, n) = 300, SHAPES[name]
+    q, s, W, _, _ = operands(dev, name, k, dtype, seed=3)
+    clean = dense_ops.fp8_matmul(q, s, W, out_dtype=dtype)
+    if torch.cuda.mem_get_info(dev)[0] < 2 * m << 23:
+        pytest.skip("not enough memory")
+    far = torch.empty(m << 23, dtype=torch.uint8, device=dev).as_strided(q.shape, (1 << 23, 1))
+    far.copy_(q.view(torch.uint8))
+    far_scale = torch.empty(m << 21, dtype=torch.float32, device=dev).as_strided(s.shape, (1 << 21, 1))
+    far_scale.copy_(s)
+    assert dense_ops.describe_fp8_matmul(m, n, dtype, 1 << 23, 1 << 21) == name
+    assert torch.equal(dense_ops.fp8_matmul(far.view(torch.float8_e4m3fn), far_scale, W, out_dtype=dtype), clean)
+
+
 def test_describe_refusals():
     import ctypes
     from nerffaceediting_amd import _lib, dense_ops
