@@ -78,7 +78,7 @@ def test_image_replaced_while_another_stream_reads_it(dev):
     torch.cuda.synchronize()
     side = torch.cuda.Stream(device=dev)
     with torch.cuda.stream(side):
-        torch.cuda._sleep(200_000_000)                                    # about 0.1 s
+        torch.cuda._sleep(1_000_000_000)                                  # about half a second
         out = layer.forward_fp8(q, s)
         done = torch.cuda.Event()
         done.record()
